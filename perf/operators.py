@@ -220,8 +220,8 @@ def plain_linear(state):
     x = state["x"].float()
     y = [x @ values(*w).T for w in state["weights"]]
     if state["case"]["kind"] == "gated":
-        return (y[0] / (1.0 + torch.exp(-y[0])) * y[1]).to(state["x"].dtype)
-    return y[0]
+        y = [y[0] / (1.0 + torch.exp(-y[0])) * y[1]]
+    return y[0].to(state["x"].dtype)
 
 
 def plain_store(state):
@@ -319,7 +319,7 @@ def run(state):
     if not state["own"]:
         return dict(linear=plain_linear, gated=plain_linear, store=plain_store, attend=plain_attend)[case["kind"]](state)
     if case["kind"] == "linear":
-        return state["product"](state["x"], out_dtype=torch.float32)
+        return state["product"](state["x"])
     if case["kind"] == "gated":
         return state["product"](state["x"], state["x"].dtype)
     nh, nkv, hd = case["nh"], case["nkv"], case["hd"]
@@ -340,7 +340,7 @@ def work(case):
     eb = 2 if case["dtype"] == "bfloat16" else 4
     if case["kind"] in ("linear", "gated"):
         M, N, K, n = case["M"], case["N"], case["K"], 2 if case["kind"] == "gated" else 1
-        return dict(bytes=n * N * K * (0.5 + 2.0 / case["group"]) + eb * M * K + M * N * (eb if n == 2 else 4),
+        return dict(bytes=n * N * K * (0.5 + 2.0 / case["group"]) + eb * M * (K + N),
                     flops=2.0 * n * M * N * K)
     nh, nkv, hd, T = case["nh"], case["nkv"], case["hd"], case["tokens"]
     row = 2 * nkv * hd * (0.5 + 2.0 / GROUP)                          # a position's key and value
