@@ -25,6 +25,7 @@ class KVLayerView:
     seq_slot: torch.Tensor          # row index into page_table (the step's seq_row)
     window: Optional[int]
     writes: bool                    # False: this run only reads what another run wrote
+    bits: int = 16                  # 4: the pools are one tensor of pages that hold keys and values in four bits (csrc/q4.cuh)
 
 
 @dataclass

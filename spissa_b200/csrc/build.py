@@ -63,6 +63,13 @@ MODULES = {
     "sandwich": "sandwich_kernels.cu",
     "rglru": "rglru_kernels.cu",
     "mlstm": "mlstm_kernels.cu",
+    "q4": "q4_kernels.cu",
+    "kv4": "kv4_kernels.cu",
+}
+# headers that only these modules include
+OWN_HEADERS = {
+    "q4_kernels.cu": ["q4.cuh"],
+    "kv4_kernels.cu": ["q4.cuh", "kv4.cuh"],
 }
 
 
@@ -116,7 +123,7 @@ def build_dir() -> Path:
 
 def _digest(source: str, range_check=None) -> str:
     h = hashlib.sha256()
-    for name in [source] + HEADERS:
+    for name in [source] + HEADERS + OWN_HEADERS.get(source, []):
         h.update(name.encode())
         h.update((CSRC / name).read_bytes())
     h.update(" ".join(flags(range_check)).encode())

@@ -1763,3 +1763,140 @@ def mlstm(proj, w: dict, state, nm, out, step, H, d, vd, cap, eps):
         dt_code(out), c_void_p(_ptr(step.seq_start)), c_void_p(_ptr(step.seq_slot)), step.n_seqs, T, n_chunks, int(H), int(d),
         int(vd), c_float(cap), c_float(eps), c_void_p(_ptr(scratch)), mode, c_void_p(_ptr(status_word(proj.device))),
         c_void_p(_stream())))
+
+
+# ------------------------------------------------------------------ four bits: weights
+def _on_one_device(what: str, *ts) -> None:
+    """A launch goes to the current device's stream: its tensors have to live there."""
+    here = torch.cuda.current_device()
+    for t in ts:
+        if t is not None and (not t.is_cuda or t.device.index != here):
+            raise KernelError(f"{what}: tensors on the current device (cuda:{here}) are wanted, got one on {t.device}")
+
+
+def q4_shapes(rows: int, K: int, group: int, half: int = 0) -> tuple:
+    """Shapes of a packed weight's codes (uint8) and scales (int16); ``half``: rows of gate and of up each, 0 for a plain weight."""
+    if K <= 0 or K % 32 or group not in (32, 64, 128) or K % group or rows <= 0:
+        raise KernelError(f"four-bit weights: rows of a multiple of 32 columns in groups of 32, 64 or 128, got {rows} x {K} in groups of {group}")
+    if half and rows != 2 * half:
+        raise KernelError(f"four-bit weights: gate and up have {half} rows each, the weight {rows}")
+    packed = (half + 15) // 16 * 32 if half else (rows + 15) // 16 * 16
+    blocks = (K + 63) // 64
+    return (packed // 16, blocks, 512), (packed // 16, blocks * 64 // group, 16)
+
+
+def q4_pack(w, group: int, half: int = 0) -> tuple:
+    """(codes, scales) of a weight [rows, K], float32 or bfloat16, in the products' layout (q4_kernels.cu); ``half``: its rows are
+    so many gate rows and then as many up rows."""
+    if w.dim() != 2 or w.stride(1) != 1:
+        raise KernelError("four-bit weights are packed from a matrix with unit stride in its last dimension")
+    _on_one_device("q4_pack", w)
+    lib = load("q4")
+    c, s = q4_shapes(w.shape[0], w.shape[1], group, half)
+    codes, scales = torch.empty(c, dtype=torch.uint8, device=w.device), torch.empty(s, dtype=torch.int16, device=w.device)
+    _check("q4", lib.sp_q4_pack(
+        c_void_p(_ptr(w)), dt_code(w), c_longlong(w.stride(0)), c_void_p(_ptr(codes)), c_void_p(_ptr(scales)), w.shape[0], w.shape[1],
+        int(group), int(half), c_void_p(_stream())))
+    return codes, scales
+
+
+def _q4_weight(what: str, codes, scales, rows: int, K: int, group: int, half: int) -> None:
+    c, s = q4_shapes(rows, K, group, half)
+    if tuple(codes.shape) != c or tuple(scales.shape) != s or codes.dtype != torch.uint8 or scales.dtype != torch.int16:
+        raise KernelError(f"{what}: codes uint8 {c} and scales int16 {s} are wanted, got {codes.dtype} {tuple(codes.shape)} and "
+                          f"{scales.dtype} {tuple(scales.shape)}")
+    _need_contig(codes, scales)
+
+
+def q4_unpack(codes, scales, out, group: int, half: int = 0, block: int = 0) -> None:
+    """``out`` [rows, K] = the numbers a packed weight stands for (each exactly a bfloat16). ``half``: gate and up rows, in ``out``
+    in turns of ``block`` (0: all gate rows, then all up rows)."""
+    rows, K = out.shape
+    _q4_weight("q4_unpack", codes, scales, rows, K, group, half)
+    _need_contig(out)
+    _on_one_device("q4_unpack", codes, scales, out)
+    _check("q4", load("q4").sp_q4_unpack(
+        c_void_p(_ptr(codes)), c_void_p(_ptr(scales)), c_void_p(_ptr(out)), dt_code(out), rows, K, int(group), int(half), int(block),
+        c_void_p(_stream())))
+
+
+# ------------------------------------------------------------------ four bits: keys and values
+KV4_HEAD_SIZES = (32, 64, 96, 128)
+
+
+def kv4_tile_bytes(hd: int) -> int:
+    """Bytes of one kv head's page (64 keys and values): codes of four bits and 16 bits for every 32 of them."""
+    if hd not in KV4_HEAD_SIZES:
+        raise KernelError(f"a four-bit cache takes heads of {', '.join(map(str, KV4_HEAD_SIZES))}, got {hd}")
+    return 64 * (hd + hd // 8)
+
+
+def kv4_pool(n_pages: int, nkv: int, hd: int, device) -> torch.Tensor:
+    """Pages of a four-bit cache, zeros: uint8 [pages, kv heads, bytes of a page]."""
+    return torch.zeros(int(n_pages), int(nkv), kv4_tile_bytes(hd), dtype=torch.uint8, device=device)
+
+
+def _kv4_check(what: str, pool, meta, T: int, nkv: int, hd: int, *ts) -> None:
+    if pool.dtype != torch.uint8 or pool.dim() != 3 or pool.shape[1] != nkv or pool.shape[2] != kv4_tile_bytes(hd):
+        raise KernelError(f"{what}: pages are uint8 [pages, {nkv}, {kv4_tile_bytes(hd)}], got {pool.dtype} {tuple(pool.shape)}")
+    if meta.page_size != 64:
+        raise KernelError(f"{what}: pages of 64 positions, got {meta.page_size}")
+    tables = (meta.token_seq, meta.positions, meta.seq_slot, meta.page_table)
+    if any(t.dtype != torch.int32 for t in tables) or meta.page_table.dim() != 2 or min(meta.token_seq.numel(), meta.positions.numel()) < T:
+        raise KernelError(f"{what}: the step's arrays are int32, one sequence and position a token, pages [sequences, entries]")
+    _need_contig(pool, *tables, *ts)
+    _on_one_device(what, pool, *tables, *ts)
+
+
+def kv4_store(qkv, q_out, pool, meta, inv_freq, nh, nkv, hd, rd, write_kv=True) -> None:
+    """Rotate q and k of ``qkv`` [T, (nh + 2·nkv)·hd] (float32) at the tokens' positions (the first ``rd`` dims of a head, dim i with
+    i + rd/2; 0: as they are), q to ``q_out`` [T, nh·hd], k and v in four bits into the pages of ``pool``. ``meta`` as
+    for ``rope_kv_write``. ``nh`` may be 0 (``q_out`` None)."""
+    T = qkv.shape[0]
+    if qkv.dtype != torch.float32 or qkv.dim() != 2 or qkv.shape[1] != (nh + 2 * nkv) * hd:
+        raise KernelError(f"kv4_store: rows of {nh} + 2 x {nkv} heads of {hd} in float32 are wanted, got {qkv.dtype} {tuple(qkv.shape)}")
+    if (q_out is None) != (nh == 0) or (q_out is not None and tuple(q_out.shape) != (T, nh * hd)):
+        raise KernelError(f"kv4_store: q goes to a tensor [{T}, {nh * hd}]")
+    if rd and (inv_freq is None or inv_freq.dtype != torch.float32 or inv_freq.numel() < rd // 2):
+        raise KernelError(f"kv4_store: rotating {rd} dims takes {rd // 2} float32 frequencies")
+    _kv4_check("kv4_store", pool, meta, T, nkv, hd, qkv, q_out, inv_freq)
+    lib = load("kv4")
+    pt = meta.page_table
+    _declare_bounds("kv4", lib, _pool_pages(meta, pool), _table_rows(meta, pt), qkv.device)
+    _check("kv4", lib.sp_kv4_store(
+        c_void_p(_ptr(qkv)), c_void_p(_ptr(q_out)), dt_code(q_out) if q_out is not None else F32, c_void_p(_ptr(pool)),
+        c_void_p(_ptr(meta.token_seq)), c_void_p(_ptr(meta.positions)), c_void_p(_ptr(meta.seq_slot)), c_void_p(_ptr(pt)), pt.shape[1],
+        meta.page_size, c_void_p(_ptr(inv_freq)), T, int(nh), int(nkv), int(hd), int(rd), int(bool(write_kv)), c_void_p(_stream())))
+
+
+def kv4_load(pool, meta, k_out, v_out, nkv, hd) -> None:
+    """k_out, v_out [T, nkv, hd] (float32 or bfloat16, which holds them exactly) = what the pages hold of the step's tokens."""
+    T = k_out.shape[0]
+    if tuple(k_out.shape) != (T, nkv, hd) or v_out.shape != k_out.shape or v_out.dtype != k_out.dtype:
+        raise KernelError(f"kv4_load: keys and values go to two tensors [tokens, {nkv}, {hd}] of one type")
+    _kv4_check("kv4_load", pool, meta, T, nkv, hd, k_out, v_out)
+    lib = load("kv4")
+    pt = meta.page_table
+    _declare_bounds("kv4", lib, _pool_pages(meta, pool), _table_rows(meta, pt), pool.device)
+    _check("kv4", lib.sp_kv4_load(
+        c_void_p(_ptr(pool)), c_void_p(_ptr(k_out)), c_void_p(_ptr(v_out)), dt_code(k_out), c_void_p(_ptr(meta.token_seq)),
+        c_void_p(_ptr(meta.positions)), c_void_p(_ptr(meta.seq_slot)), c_void_p(_ptr(pt)), pt.shape[1], meta.page_size, T, int(nkv),
+        int(hd), c_void_p(_stream())))
+
+
+def kv4_unpack_pages(pool, meta, k_out, v_out, table, step, window, nkv, hd) -> None:
+    """k_out, v_out [pages, nkv, 64, hd] = the numbers in the pages of the step's sequences, one sequence after another; ``table``
+    (int32, as ``meta.page_table``) = which page went where. Positions behind a sequence's end are zeros; pages that no
+    query's ``window`` reaches keep what they hold."""
+    pt = meta.page_table
+    if table.dtype != torch.int32 or table.shape != pt.shape or k_out.shape != v_out.shape or k_out.dtype != v_out.dtype \
+            or tuple(k_out.shape[1:]) != (nkv, 64, hd):
+        raise KernelError(f"kv4_unpack_pages: two pools [pages, {nkv}, 64, {hd}] of one type and a table like the cache's are wanted")
+    _kv4_check("kv4_unpack_pages", pool, meta, 0, nkv, hd, k_out, v_out, table, step.seq_len, step.seq_start)
+    lib = load("kv4")
+    _declare_bounds("kv4", lib, _pool_pages(meta, pool), _table_rows(meta, pt), pool.device)
+    _check("kv4", lib.sp_kv4_unpack_pages(
+        c_void_p(_ptr(pool)), c_void_p(_ptr(k_out)), c_void_p(_ptr(v_out)), dt_code(k_out), c_void_p(_ptr(table)),
+        c_void_p(_ptr(step.seq_len)), c_void_p(_ptr(step.seq_start)), c_void_p(_ptr(meta.positions)), int(window or 0),
+        c_void_p(_ptr(meta.seq_slot)), c_void_p(_ptr(pt)), pt.shape[1], meta.page_size, int(step.n_seqs), k_out.shape[0], int(nkv), int(hd),
+        c_void_p(_stream())))

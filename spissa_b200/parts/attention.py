@@ -19,6 +19,7 @@ import math
 
 import torch
 
+from ..cache.views import KVLayerView
 from ..csrc import lib as K
 from .base import KVCacheRequest, Mixer, WeightSpec
 from .linear import GEMV_TOKENS, Linear
@@ -166,6 +167,10 @@ def attend_paged(q, step, cache, nh, nkv, hd, window, scale, sink=None, counters
     T = q.shape[0]
     if vd == hd:
         vd = None
+    if getattr(cache, "bits", 16) == 4:
+        if vd is not None or dist_bias is not None:
+            raise K.KernelError("attention over a four-bit cache takes key and value rows of one size and no scores by distance")
+        return attend_four_bits(q, step, cache, nh, nkv, hd, window, scale, sink)
     ctx = torch.empty_like(q) if vd is None else torch.empty(T, nh * vd, dtype=q.dtype, device=q.device)
     if vd is None and K.flash_supported(q, cache.k_pool, nh, nkv, hd, cache.page_size):
         flash = {}
@@ -203,3 +208,19 @@ def attend_paged(q, step, cache, nh, nkv, hd, window, scale, sink=None, counters
         K.flash_prefill(q, cache.k_pool, cache.v_pool, ctx, cache, step.seq_start, step.n_seqs,
                         tiles, nh, nkv, hd, window, scale, sink=sink, dist_bias=dist_bias, **flash)
     return ctx
+
+
+def attend_four_bits(q, step, cache, nh, nkv, hd, window, scale, sink=None):
+    """``attend_paged`` over pages of four bits."""
+    T = q.shape[0]
+    if q.dtype not in (torch.bfloat16, torch.float32) or tuple(q.shape) != (T, nh * hd) or nh % nkv:
+        raise K.KernelError(f"attention: queries are [tokens, {nh} x {hd}], bfloat16 or float32, of heads in equal groups")
+    lens = step.host.get("seq_len") or step.seq_len.tolist()
+    n_pages = sum(-(-n // cache.page_size) for n in lens)
+    k = torch.empty(n_pages, nkv, cache.page_size, hd, dtype=q.dtype, device=q.device)
+    v = torch.empty_like(k)
+    table = torch.empty_like(cache.page_table)
+    K.kv4_unpack_pages(cache.k_pool, cache, k, v, table, step, window, nkv, hd)
+    rows = torch.arange(step.n_seqs, dtype=torch.int32, device=q.device)
+    plain = KVLayerView(k, v, table, cache.page_size, cache.token_seq, cache.positions, rows, cache.window, False)
+    return attend_paged(q, step, plain, nh, nkv, hd, window, scale, sink)

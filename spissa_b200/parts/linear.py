@@ -6,6 +6,10 @@ kernel for a few tokens (decoding), to the tcgen05 kernel with the weight's rows
 to some hundreds of tokens, and to the tcgen05 tile kernel otherwise, when the rows are multiples of 16 bytes;
 32-bit products of more than ``GEMV_TOKENS`` rows go to the tcgen05 kernel that multiplies float32 in bfloat16 parts;
 everything else goes to the FFMA kernels.
+
+``Linear4`` and ``GatedLinear4`` hold their weights in four bits with a scale for every ``group`` columns (not in the
+reference; csrc/q4.cuh states the format): the numbers that stand in their place are exactly bfloat16, and all their
+products multiply those.
 """
 from __future__ import annotations
 
@@ -147,3 +151,73 @@ class GatedLinear:
             gu = self.plain(x, out_dtype=act_dtype)
             K.gated_mul(gu, out, self.act, self.mult)
         return out
+
+
+class Linear4:
+    """y = x · Ŵᵀ, Ŵ the numbers that ``weight`` [out, in] becomes in four bits, in groups of ``group`` (32, 64 or 128) columns;
+    in a multiple of the group. Called as ``Linear``: x bfloat16 or float32."""
+
+    def __init__(self, weight: torch.Tensor, group: int = 64):
+        if weight.dim() != 2:
+            raise ValueError("a linear weight is a matrix [out, in]")
+        self.out_features, self.in_features = weight.shape
+        self.group = int(group)
+        self.codes, self.scales = K.q4_pack(weight.contiguous(), self.group)
+
+    def unpacked(self, dtype=torch.bfloat16) -> torch.Tensor:
+        w = torch.empty(self.out_features, self.in_features, dtype=dtype, device=self.codes.device)
+        K.q4_unpack(self.codes, self.scales, w, self.group)
+        return w
+
+    def __call__(self, x: torch.Tensor, out: torch.Tensor | None = None, out_dtype=None,
+                 accumulate: bool = False) -> torch.Tensor:
+        """``accumulate`` adds the product into ``out`` (float32) instead of overwriting it."""
+        if out is None:
+            if accumulate:
+                raise ValueError("accumulation needs the tensor to add into")
+            out = torch.empty(x.shape[0], self.out_features, dtype=out_dtype or x.dtype, device=x.device)
+        check4(x, self.in_features, out, self.out_features, accumulate)
+        if x.shape[0]:
+            Linear(self.unpacked(x.dtype))(x, out=out, accumulate=accumulate)
+        return out
+
+
+class GatedLinear4:
+    """act(x·Ŵgᵀ) ⊙ (x·Ŵuᵀ) · mult with gate and up weights in four bits (``act``: K.ACT_SILU or K.ACT_GELU)."""
+
+    def __init__(self, gate: torch.Tensor, up: torch.Tensor, act: int = K.ACT_SILU, mult: float = 1.0, group: int = 64):
+        if gate.dim() != 2 or gate.shape != up.shape or gate.dtype != up.dtype:
+            raise ValueError("gate and up weights are two matrices [out, in] of one type")
+        if act not in (K.ACT_SILU, K.ACT_GELU):
+            raise ValueError("gated products of four-bit weights are built for silu and gelu")
+        self.act, self.mult, self.group = act, float(mult), int(group)
+        self.intermediate, self.in_features = gate.shape
+        self.codes, self.scales = K.q4_pack(torch.cat([gate, up], dim=0), self.group, half=self.intermediate)
+
+    def unpacked(self, dtype=torch.bfloat16) -> GatedLinear:
+        """The product over the numbers the codes stand for."""
+        plain = GatedLinear.__new__(GatedLinear)
+        I = self.intermediate
+        plain.act, plain.mult, plain.limit, plain.slope, plain.intermediate = self.act, self.mult, 0.0, 0.0, I
+        plain.block = 0 if dtype != torch.bfloat16 else 128 if I % 128 == 0 else 64 if I % 64 == 0 else 0
+        plain.weight = torch.empty(2 * I, self.in_features, dtype=dtype, device=self.codes.device)
+        K.q4_unpack(self.codes, self.scales, plain.weight, self.group, half=I, block=plain.block)
+        plain.plain = Linear(plain.weight)
+        return plain
+
+    def __call__(self, x: torch.Tensor, act_dtype) -> torch.Tensor:
+        out = torch.empty(x.shape[0], self.intermediate, dtype=act_dtype, device=x.device)
+        check4(x, self.in_features, out, self.intermediate, False)
+        return self.unpacked(x.dtype)(x, act_dtype) if x.shape[0] else out
+
+
+def check4(x, in_features: int, out, out_features: int, accumulate: bool) -> None:
+    """Refuses what the products of four-bit weights do not take."""
+    if x.dtype not in (torch.bfloat16, torch.float32):
+        raise K.KernelError(f"products of four-bit weights take bfloat16 or float32 rows, got {x.dtype}")
+    if x.dim() != 2 or x.shape[1] != in_features or tuple(out.shape) != (x.shape[0], out_features):
+        raise K.KernelError(f"shapes do not match: x {tuple(x.shape)}, weight [{out_features}, {in_features}], out {tuple(out.shape)}")
+    if x.stride(1) != 1 or out.stride(1) != 1:
+        raise K.KernelError("product operands must have unit stride in their last dimension")
+    if out.dtype not in (torch.bfloat16, torch.float32) or (accumulate and out.dtype != torch.float32):
+        raise K.KernelError(f"products are stored as bfloat16 or float32 and added into float32, got {out.dtype}")
