@@ -43,6 +43,10 @@ def load(module: str) -> ctypes.CDLL:
         except OSError as e:
             raise KernelError(f"cannot load kernel library {path}: {e}") from None
         getattr(lib, f"sp_{module}_last_error").restype = ctypes.c_char_p
+        if module == "q4":
+            # declared once: plain integers pass, without an object made for each of a call's arguments
+            lib.sp_q4_gemv.argtypes = [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_longlong,
+                                       c_longlong, c_int, c_int, c_float, c_void_p]
         if module == "seqmix":
             lib.sp_retention_chunked_scratch_floats.restype = c_longlong
         if module == "mlstm":
@@ -1818,6 +1822,20 @@ def q4_unpack(codes, scales, out, group: int, half: int = 0, block: int = 0) -> 
     _check("q4", load("q4").sp_q4_unpack(
         c_void_p(_ptr(codes)), c_void_p(_ptr(scales)), c_void_p(_ptr(out)), dt_code(out), rows, K, int(group), int(half), int(block),
         c_void_p(_stream())))
+
+
+Q4_GEMV_ROWS = 16         # rows of x that ``q4_gemv`` takes
+
+
+def q4_gemv(x, codes, scales, out, rows: int, group: int, half: int = 0, mode=TC_STORE, act=ACT_SILU, mult: float = 1.0) -> None:
+    """out = x · Ŵᵀ for up to 16 rows of x, streaming the codes once. Modes as ``tc_gemm``; TC_SILU_MUL with ``half`` gate rows. The
+    caller has checked the shapes (``parts.linear.check4``); rows of ``x`` start on 16-byte boundaries."""
+    lib = load("q4")
+    M, K = x.shape
+    rc = lib.sp_q4_gemv(x.data_ptr(), dt_code(x), codes.data_ptr(), scales.data_ptr(), out.data_ptr(), dt_code(out), M, rows, K, group, half,
+                        x.stride(0), out.stride(0), mode, act, mult, _stream())
+    if rc:
+        _check("q4", rc)
 
 
 # ------------------------------------------------------------------ four bits: keys and values
