@@ -1785,8 +1785,8 @@ def q4_shapes(rows: int, K: int, group: int, half: int = 0) -> tuple:
     if half and rows != 2 * half:
         raise KernelError(f"four-bit weights: gate and up have {half} rows each, the weight {rows}")
     packed = (half + 15) // 16 * 32 if half else (rows + 15) // 16 * 16
-    blocks = (K + 63) // 64
-    return (packed // 16, blocks, 512), (packed // 16, blocks * 64 // group, 16)
+    blocks = (K + 127) // 128
+    return (packed // 16, blocks, 1024), (packed // 16, blocks, 8, 128 // group, 2)
 
 
 def q4_pack(w, group: int, half: int = 0) -> tuple:

@@ -1,10 +1,12 @@
 // Weights of four bits (q4.cuh): packing, unpacking, and the product for up to 16 tokens.
 //
-// Layout. Rows of W come in tiles of 16, columns in blocks of 64, both filled up with zeros. A block of a tile is 512 bytes:
-// lane 4 g + t of a warp owns 16 of them, the words (row g: columns 8 t.., 32 + 8 t..), (row g + 8: the same), that
-// is, the A operand of four m16n8k16 products in one load. Scales and zeros: [tile][group of columns][16 rows], 16 bits each.
-// A gated product's rows alternate by tiles: 16 gate rows, the 16 up rows of the same outputs.
+// Layout. Rows of W come in tiles of 16, columns in blocks of 128, both filled up with zeros. A block of a tile is 1,024 bytes, two
+// pieces of 64 columns: lane 4 g + t of a warp owns 16 bytes of each, the words (row g: columns 8 t.., 32 + 8 t..), (row g + 8:
+// the same), that is, the A operand of four m16n8k16 products in one load. Scales and zeros: [tile][block][row g][group of the
+// block][row g, row g + 8], 16 bits each. A gated product's rows alternate by tiles: 16 gate rows, the 16 up rows of the same
+// outputs.
 #include "q4.cuh"
+#include <cuda_fp16.h>
 
 SP_API const char* sp_q4_last_error() { return sp_error_text; }
 SP_DEFINE_RANGE_API(q4)
@@ -21,17 +23,22 @@ __device__ __forceinline__ int source_row(int packed, int rows, const RowMap& m)
     return m.block ? (o / m.block) * 2 * m.block + up * m.block + o % m.block : up * m.half + o;
 }
 
-__device__ __forceinline__ size_t word_at(int row, int k8, int kblocks) {            // the word of columns 8 k8 .. of a packed row
-    const int kb = k8 >> 3, t = k8 & 3, h = (k8 >> 2) & 1;
-    return (((size_t)(row >> 4) * kblocks + kb) * 32 + (row & 7) * 4 + t) * 4 + ((row >> 3) & 1) * 2 + h;
+constexpr int BLOCK = 128;         // columns
+
+__device__ __forceinline__ size_t word_at(int row, int k8, int blocks) {             // the word of columns 8 k8 .. of a packed row
+    return ((((size_t)(row >> 4) * blocks + (k8 >> 4)) * 2 + ((k8 >> 3) & 1)) * 32 + (row & 7) * 4 + (k8 & 3)) * 4 + ((row >> 3) & 1) * 2 + ((k8 >> 2) & 1);
+}
+__device__ __forceinline__ size_t meta_at(int row, int k8, int blocks, int group) {
+    const int per = BLOCK / group;
+    return ((((size_t)(row >> 4) * blocks + (k8 >> 4)) * 8 + (row & 7)) * per + (8 * k8 % BLOCK) / group) * 2 + ((row >> 3) & 1);
 }
 
 // A thread packs eight columns of a row; 4, 8 or 16 neighbouring threads share a group.
-__global__ void pack_kernel(const void* w, int dt, long long ldw, uint32_t* codes, uint16_t* meta, int rows, int K, int kblocks,
+__global__ void pack_kernel(const void* w, int dt, long long ldw, uint32_t* codes, uint16_t* meta, int rows, int K, int blocks,
                             int group, RowMap map) {
     const int row = blockIdx.x, k8 = blockIdx.y * blockDim.x + threadIdx.x;
     const int src = source_row(row, rows, map);
-    const bool in = src >= 0 && 8 * k8 < K;
+    const bool in = src >= 0 && 8 * k8 < K, kept = k8 < blocks * 16;
     float x[8], lo = 0.0f, hi = 0.0f;
     bool bad = false;
 #pragma unroll
@@ -51,18 +58,18 @@ __global__ void pack_kernel(const void* w, int dt, long long ldw, uint32_t* code
     uint32_t word = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) word |= (uint32_t)q4_code(x[i], g) << (4 * (i / 2 + 4 * (i & 1)));
-    if (k8 >= kblocks * 8) return;
-    codes[word_at(row, k8, kblocks)] = word;
-    if ((8 * k8) % group == 0) meta[((size_t)(row >> 4) * (kblocks * 64 / group) + 8 * k8 / group) * 16 + (row & 15)] = (uint16_t)q4_meta(g);
+    if (!kept) return;
+    codes[word_at(row, k8, blocks)] = word;
+    if ((8 * k8) % group == 0) meta[meta_at(row, k8, blocks, group)] = (uint16_t)q4_meta(g);
 }
 
 template <typename T>
-__global__ void unpack_kernel(const uint32_t* codes, const uint16_t* meta, T* out, int rows, int K, int kblocks, int group, RowMap map) {
+__global__ void unpack_kernel(const uint32_t* codes, const uint16_t* meta, T* out, int rows, int K, int blocks, int group, RowMap map) {
     const int row = blockIdx.x, k8 = blockIdx.y * blockDim.x + threadIdx.x;
     const int dst = source_row(row, rows, map);
     if (dst < 0 || 8 * k8 >= K) return;
-    const uint32_t word = codes[word_at(row, k8, kblocks)];
-    const uint32_t m = meta[((size_t)(row >> 4) * (kblocks * 64 / group) + 8 * k8 / group) * 16 + (row & 15)];
+    const uint32_t word = codes[word_at(row, k8, blocks)];
+    const uint32_t m = meta[meta_at(row, k8, blocks, group)];
     T* to = out + (size_t)dst * K + 8 * k8;
 #pragma unroll
     for (int i = 0; i < 8; i += 2)
@@ -70,50 +77,45 @@ __global__ void unpack_kernel(const uint32_t* codes, const uint16_t* meta, T* ou
 }
 
 // ---------------------------------------------------------------- the product for a few tokens
-// out[M, N] = x[M, K] · Ŵ[N, K]ᵀ, M <= 16, bound by streaming the codes once.
+// out[M, N] = x[M, K] · Ŵ[N, K]ᵀ, M <= 16, bound by streaming the codes once; what stands in the way is instructions, so the
+// number type is the one that takes the fewest to pull a code out of its word: the four bits in the lowest place of a half word
+// ARE the float16 c · 2^-24, one place up 16 c · 2^-24, so w & 0x000f000f and w & 0x00f000f0 are operands of m16n8k16, and w >> 8
+// holds the next two pairs (tensor cores take subnormal numbers as any other). (As e4m3 numbers a code is c · 2^-9 and takes
+// half of that, but m16n8k32 on those runs at half the rate of two on float16 here.)
+// x is multiplied by a power of two per row and block of 128 columns that brings the block's largest entry into 2^14 .. 2^15:
+// exact for bfloat16 entries down to 2^-26 of the block's largest, off by 2^-39 of the largest below. float32 entries are two
+// float16 numbers each, 22 bits. (Blocks whose largest entry lies outside 2^-80 .. 2^100 overflow or vanish.) The zero is taken off
+// the sums, Σ x (c − z) = Σ x c − z Σ x, with Σ x per group in 32 bits, and a group's sum is scaled in 32 bits. A row with
+// an entry that is not finite gives NaN.
 //
-// A CTA owns two tiles of 16 rows (gated: 16 gate rows and the up rows of the same outputs); its warps, and the CTAs of a cluster,
-// share the blocks of K. Per block of 64 a lane loads 16 bytes of codes per tile and 32 of x per eight tokens, and four
-// mma.sync m16n8k16 multiply the codes less their zero (c − z, exact in bfloat16) with x as the columns. A
-// group's sum is scaled in 32 bits and added to the row's: no rounding but the sums' own. float32 rows are taken apart into
-// three bfloat16 parts, 8 bits of the mantissa each, and each part is multiplied: the same sums, exactly x.
-// Partial sums are added in the order of the warps, then of the CTAs, so a row's result depends neither on timing nor on M.
+// x stands still: a warp owns a block of columns, whose x it holds in registers as the operands want it, and walks over
+// tiles of 16 rows, fetching the next codes while it multiplies. So shared memory, whose 128 bytes a cycle the codes alone
+// would half fill, takes one partial sum a tile and block; warps of a CTA and CTAs of a cluster share K, and at the end
+// their sums are added in order: a row's result depends neither on timing nor on the other rows.
 enum { MODE_STORE = 0, MODE_ACCUMULATE = 1, MODE_SILU_MUL = 2 };
-constexpr int WARPS = 8;
 
-__device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint4 ld_once(const uint4* p) {           // codes: read once, not kept in L1
-    uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-    return v;
-}
 
-// The bfloat16 pairs of eight neighbouring entries of a row of x, in one part or in three.
-__device__ __forceinline__ void x_pairs(const __nv_bfloat16* p, bool ok, uint32_t (&out)[1][4]) {
-    const uint4 v = ok ? *(const uint4*)p : make_uint4(0, 0, 0, 0);
-    out[0][0] = v.x; out[0][1] = v.y; out[0][2] = v.z; out[0][3] = v.w;
+__device__ __forceinline__ float finite_or_nan(float v) { return fabsf(v) < INFINITY ? v : __int_as_float(0x7fc00000); }
+__device__ __forceinline__ void load8(const __nv_bfloat16* p, bool ok, float (&v)[8]) {
+    const uint4 w = ok ? *(const uint4*)p : make_uint4(0, 0, 0, 0);
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { v[2 * i] = finite_or_nan(__uint_as_float(u[i] << 16)); v[2 * i + 1] = finite_or_nan(__uint_as_float(u[i] & 0xffff0000u)); }
 }
-__device__ __forceinline__ void x_pairs(const float* p, bool ok, uint32_t (&out)[3][4]) {
-    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (ok) {
-        *(float4*)v = *(const float4*)p;
-        *(float4*)(v + 4) = *(const float4*)(p + 4);
-    }
+__device__ __forceinline__ void load8(const float* p, bool ok, float (&v)[8]) {
+    const float4 a = ok ? *(const float4*)p : make_float4(0.f, 0.f, 0.f, 0.f), b = ok ? *(const float4*)(p + 4) : a;
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
 #pragma unroll
-    for (int part = 0; part < 3; ++part)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t a = __float_as_uint(v[2 * i]), b = __float_as_uint(v[2 * i + 1]);
-            out[part][i] = __byte_perm(a, b, 0x7632);
-            v[2 * i] -= __uint_as_float(a & 0xffff0000u);
-            v[2 * i + 1] -= __uint_as_float(b & 0xffff0000u);
-            if (v[2 * i] != v[2 * i]) v[2 * i] = 0.0f;               // an infinity is its first part
-            if (v[2 * i + 1] != v[2 * i + 1]) v[2 * i + 1] = 0.0f;
-        }
+    for (int i = 0; i < 8; ++i) v[i] = finite_or_nan(v[i]);
+}
+__device__ __forceinline__ uint32_t half2_of(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *(const uint32_t*)&h;
 }
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -124,182 +126,262 @@ __device__ __forceinline__ uint32_t cluster_rank() {
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ float4 ld_peer(const void* local, uint32_t rank) {
+__device__ __forceinline__ float4 ld_peer(const float4* local, uint32_t rank) {
     uint32_t ra;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(ra) : "r"((uint32_t)__cvta_generic_to_shared(local)), "r"(rank));
     float4 v;
     asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(ra) : "memory");
     return v;
 }
-
-struct Product {
-    const uint4* codes;
-    const uint16_t* meta;
-    void* out;
-    long long ldx, ldo;
-    int out_dt, M, rows, tiles, kblocks, K, group, mode, half, cs;
-    SpGate ga;
-};
-
-template <typename TX, int NT, bool G32>
-__global__ void __launch_bounds__(WARPS * 32)
-gemv_kernel(const TX* x, const Product p) {
-    constexpr int PARTS = sizeof(TX) == 4 ? 3 : 1, RT = 2, UNROLL = NT * PARTS > 1 ? 2 : 4;
-    __shared__ __align__(16) float4 red[WARPS][RT][NT][32];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int rank = p.cs > 1 ? (int)cluster_rank() : 0, pair = blockIdx.x / p.cs;
-    const int slices = WARPS * p.cs, slice = rank * WARPS + warp;
-    const int kb0 = (int)((long long)p.kblocks * slice / slices), kb1 = (int)((long long)p.kblocks * (slice + 1) / slices);
-    const int mgroups = p.kblocks * 64 / p.group, shift = p.group == 128 ? 1 : 0;
-
-    const uint4* code[RT];
-    const uint16_t* meta[RT];
-#pragma unroll
-    for (int r = 0; r < RT; ++r) {
-        const int tile = min(pair * RT + r, p.tiles - 1);            // an odd last tile is computed twice, stored once
-        code[r] = p.codes + (size_t)tile * p.kblocks * 32 + lane;
-        meta[r] = p.meta + (size_t)tile * mgroups * 16 + g;
-    }
-    const TX* row[NT];
-    bool have[NT];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        have[n] = n * 8 + g < p.M;
-        row[n] = x + (size_t)(have[n] ? n * 8 + g : 0) * p.ldx + 8 * t;
-    }
-    float y[RT][NT][4];
-#pragma unroll
-    for (int r = 0; r < RT; ++r)
-#pragma unroll
-        for (int n = 0; n < NT; ++n) y[r][n][0] = y[r][n][1] = y[r][n][2] = y[r][n][3] = 0.0f;
-
-    for (int kb = kb0; kb < kb1; kb += UNROLL) {
-        uint4 w[UNROLL][RT];
-        uint32_t m[UNROLL][RT][G32 ? 4 : 2];
-#pragma unroll
-        for (int u = 0; u < UNROLL; ++u) {
-            const int b = min(kb + u, kb1 - 1);
-#pragma unroll
-            for (int r = 0; r < RT; ++r) {
-                w[u][r] = ld_once(code[r] + (size_t)b * 32);
-                const uint16_t* at = meta[r] + (size_t)(G32 ? 2 * b : b >> shift) * 16;
-                m[u][r][0] = __ldg(at);
-                m[u][r][1] = __ldg(at + 8);
-                if (G32) {
-                    m[u][r][G32 ? 2 : 0] = __ldg(at + 16);
-                    m[u][r][G32 ? 3 : 1] = __ldg(at + 24);
-                }
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < UNROLL; ++u) {
-            const int b = kb + u;
-            if (b >= kb1) break;
-            uint32_t xb[NT][2][PARTS][4];                            // [half of the block]
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    x_pairs(row[n] + (size_t)b * 64 + 32 * h, have[n] && (h == 0 || b * 64 + 32 < p.K), xb[n][h]);
-#pragma unroll
-            for (int r = 0; r < RT; ++r) {
-                float acc[NT][4];
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const uint32_t m0 = m[u][r][G32 ? 2 * h : 0], m1 = m[u][r][G32 ? 2 * h + 1 : 1];
-                    if (h == 0 || G32)
-#pragma unroll
-                        for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.0f;
-                    const uint32_t z0 = 0x43004300u | (m0 & 15u) * 0x10001u, z1 = 0x43004300u | (m1 & 15u) * 0x10001u;
-                    const uint32_t w0 = h ? w[u][r].y : w[u][r].x, w1 = h ? w[u][r].w : w[u][r].z;
-#pragma unroll
-                    for (int s = 0; s < 2; ++s) {
-                        const uint32_t a0 = bf2_sub(q4_pair(w0, 2 * s), z0), a1 = bf2_sub(q4_pair(w1, 2 * s), z1);
-                        const uint32_t a2 = bf2_sub(q4_pair(w0, 2 * s + 1), z0), a3 = bf2_sub(q4_pair(w1, 2 * s + 1), z1);
-#pragma unroll
-                        for (int n = 0; n < NT; ++n)
-#pragma unroll
-                            for (int q = PARTS - 1; q >= 0; --q) mma_bf16(acc[n], a0, a1, a2, a3, xb[n][h][q][2 * s], xb[n][h][q][2 * s + 1]);
-                    }
-                    if (h == 1 || G32) {
-                        const float s0 = q4_scale_of(m0), s1 = q4_scale_of(m1);
-#pragma unroll
-                        for (int n = 0; n < NT; ++n) {
-                            y[r][n][0] = fmaf(s0, acc[n][0], y[r][n][0]);
-                            y[r][n][1] = fmaf(s0, acc[n][1], y[r][n][1]);
-                            y[r][n][2] = fmaf(s1, acc[n][2], y[r][n][2]);
-                            y[r][n][3] = fmaf(s1, acc[n][3], y[r][n][3]);
-                        }
-                    }
-                }
-            }
-        }
-    }
-#pragma unroll
-    for (int r = 0; r < RT; ++r)
-#pragma unroll
-        for (int n = 0; n < NT; ++n) red[warp][r][n][lane] = make_float4(y[r][n][0], y[r][n][1], y[r][n][2], y[r][n][3]);
-    __syncthreads();
-    // the warps' sums, a thread per four values; then the cluster's
-    const bool mine = threadIdx.x < NT * 32;
-    const int n = threadIdx.x >> 5;
-    float4 sum[RT];
-    if (mine) {
-#pragma unroll
-        for (int r = 0; r < RT; ++r) {
-            sum[r] = red[0][r][n][lane];
-#pragma unroll
-            for (int o = 1; o < WARPS; ++o) {
-                const float4 v = red[o][r][n][lane];
-                sum[r].x += v.x; sum[r].y += v.y; sum[r].z += v.z; sum[r].w += v.w;
-            }
-            red[0][r][n][lane] = sum[r];
-        }
-    }
-    if (p.cs > 1) {
-        cluster_sync();
-        if (rank == 0 && mine) {
-            for (int o = 1; o < p.cs; ++o)
-#pragma unroll
-                for (int r = 0; r < RT; ++r) {
-                    const float4 v = ld_peer(&red[0][r][n][lane], o);
-                    sum[r].x += v.x; sum[r].y += v.y; sum[r].z += v.z; sum[r].w += v.w;
-                }
-        }
-        cluster_sync();                                              // nobody leaves before its sums are read
-        if (rank != 0) return;
-    }
-    if (!mine) return;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const int token = n * 8 + 2 * t + (e & 1), at = g + (e & 2 ? 8 : 0);
-        if (token >= p.M) continue;
-        const float a = e == 0 ? sum[0].x : e == 1 ? sum[0].y : e == 2 ? sum[0].z : sum[0].w;
-        const float b = e == 0 ? sum[1].x : e == 1 ? sum[1].y : e == 2 ? sum[1].z : sum[1].w;
-        if (p.mode == MODE_SILU_MUL) {
-            const int o = pair * 16 + at;
-            if (o < p.half) sp_st_dt(p.out, p.out_dt, (size_t)token * p.ldo + o, sp_gated(a, b, p.ga));
-            continue;
-        }
-#pragma unroll
-        for (int r = 0; r < RT; ++r) {
-            const int o = (pair * RT + r) * 16 + at;
-            if (o >= p.rows) continue;
-            const size_t i = (size_t)token * p.ldo + o;
-            if (p.mode == MODE_ACCUMULATE) ((float*)p.out)[i] += r ? b : a;
-            else sp_st_dt(p.out, p.out_dt, i, r ? b : a);
-        }
+__device__ __forceinline__ uint4 ld_once(const uint8_t* p) {         // codes: read once, not kept in L1
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+template <int WORDS> __device__ __forceinline__ void ld_words(const uint8_t* p, uint32_t (&m)[WORDS]) {
+    if constexpr (WORDS == 4) {
+        const uint4 v = __ldg((const uint4*)p);
+        m[0] = v.x; m[1] = v.y; m[2] = v.z; m[3] = v.w;
+    } else if constexpr (WORDS == 2) {
+        const uint2 v = __ldg((const uint2*)p);
+        m[0] = v.x; m[1] = v.y;
+    } else {
+        m[0] = __ldg((const uint32_t*)p);
     }
 }
 
+struct Product {
+    const uint8_t* codes;
+    const uint8_t* meta;
+    void* out;
+    long long ldx, ldo;
+    int out_dt, M, rows, tiles, blocks, K, mode, half;
+    int cs, ki, sets, tpc;         // CTAs of a cluster and warps of a CTA that share K, such sets of warps in a CTA, tiles of a CTA
+    SpGate ga;
+};
+
+constexpr int MOST_WARPS = 16;
+
+template <typename TX, int NT, int GROUP, int RT, int DEPTH>
+__global__ void __launch_bounds__(MOST_WARPS * 32)
+gemv_kernel(const TX* x, const Product p) {
+    constexpr int PARTS = sizeof(TX) == 4 ? 2 : 1, GROUPS = BLOCK / GROUP, META = 4 * GROUPS;        // META: bytes of a lane row's scales
+    extern __shared__ __align__(16) float4 red[];                    // [tile][share][column group][lane]
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, warps = p.sets * p.ki;
+    const int rank = p.cs > 1 ? (int)cluster_rank() : 0, set = warp / p.ki, share = warp % p.ki;
+    const int cta_tile = (blockIdx.x / p.cs) * p.tpc, n_tiles = min(p.tpc, p.tiles - cta_tile);
+    const int c0 = (int)((long long)p.blocks * rank / p.cs), c1 = (int)((long long)p.blocks * (rank + 1) / p.cs);      // the CTA's blocks
+
+    for (int b = c0 + share; b == c0 + share || b < c1; b += p.ki) {
+        const bool there = b < c1;                                   // (a CTA may have fewer blocks than shares: zeros)
+        const uint8_t* code = p.codes + ((size_t)(cta_tile + set * RT) * p.blocks + b) * 1024 + lane * 16;
+        const uint8_t* meta = p.meta + ((size_t)(cta_tile + set * RT) * p.blocks + b) * (8 * META) + g * META;
+        uint4 w[DEPTH][RT][2];
+        uint32_t m[DEPTH][RT][GROUPS];
+        int asked = set * RT;
+        auto ask = [&](int i) {
+#pragma unroll
+            for (int r = 0; r < RT; ++r)
+                if (there && asked + r < n_tiles) {
+                    w[i][r][0] = ld_once(code + (size_t)r * p.blocks * 1024);
+                    w[i][r][1] = ld_once(code + (size_t)r * p.blocks * 1024 + 512);
+                    ld_words<GROUPS>(meta + (size_t)r * p.blocks * (8 * META), m[i][r]);
+                }
+            asked += p.sets * RT;
+            code += (size_t)p.sets * RT * p.blocks * 1024;
+            meta += (size_t)p.sets * RT * p.blocks * (8 * META);
+        };
+#pragma unroll
+        for (int i = 0; i < DEPTH; ++i) ask(i);
+
+        // x of this block: lane (row g, columns 32 q + 8 t ..), eight rows at a time
+        uint4 xv[NT][4][PARTS];
+        float2 by[NT], sx[NT][GROUPS];                               // of rows 2 t and 2 t + 1
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const int token = n * 8 + g;
+            const TX* row = x + (size_t)min(token, p.M - 1) * p.ldx + (size_t)b * BLOCK + 8 * t;
+            float v[4][8], top = 0.0f;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                load8(row + 32 * q, there && token < p.M && b * BLOCK + 32 * q < p.K, v[q]);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[q][e]));                        // (NaN is left out)
+            }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const int up = top > 0.0f ? min(94, max(-94, 141 - (int)(__float_as_uint(top) >> 23))) : 0;
+            const float scale = __uint_as_float((uint32_t)(127 + up) << 23), unit = __uint_as_float((uint32_t)(151 - up) << 23);
+            by[n] = make_float2(__shfl_sync(0xffffffffu, unit, 8 * t), __shfl_sync(0xffffffffu, unit, 8 * t + 4));
+            float sum = 0.0f;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                uint32_t h[PARTS][4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float lo = v[q][2 * j] * scale, hi = v[q][2 * j + 1] * scale, f = j & 1 ? 0.0625f : 1.0f;
+                    sum += lo + hi;
+                    h[0][j] = half2_of(lo * f, hi * f);
+                    if (PARTS == 2) {
+                        const float2 first = __half22float2(*(const __half2*)&h[0][j]);
+                        h[PARTS - 1][j] = half2_of(lo * f - first.x, hi * f - first.y);
+                    }
+                }
+#pragma unroll
+                for (int part = 0; part < PARTS; ++part) xv[n][q][part] = make_uint4(h[part][0], h[part][1], h[part][2], h[part][3]);
+                if ((q + 1) % (GROUP / 32) == 0) {
+                    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                    sum *= -5.9604644775390625e-8f;                  // −2^-24 Σ x: in the units of the codes' products
+                    sx[n][q / (GROUP / 32)] = make_float2(__shfl_sync(0xffffffffu, sum, 8 * t), __shfl_sync(0xffffffffu, sum, 8 * t + 4));
+                    sum = 0.0f;
+                }
+            }
+        }
+
+        for (int j0 = set * RT; j0 < n_tiles; j0 += DEPTH * RT * p.sets) {
+#pragma unroll
+            for (int d = 0; d < DEPTH; ++d) {
+                const int j = j0 + d * RT * p.sets;
+                if (j >= n_tiles) break;
+                float4 y[RT][NT];
+#pragma unroll
+                for (int r = 0; r < RT; ++r)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) y[r][n] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (there) {
+                    float acc[RT][NT][4];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        if (q % (GROUP / 32) == 0)
+#pragma unroll
+                            for (int r = 0; r < RT; ++r)
+#pragma unroll
+                                for (int n = 0; n < NT; ++n) acc[r][n][0] = acc[r][n][1] = acc[r][n][2] = acc[r][n][3] = 0.0f;
+#pragma unroll
+                        for (int half = 0; half < 2; ++half)
+#pragma unroll
+                            for (int r = 0; r < RT; ++r) {
+                                const uint4 c = w[d][r][q >> 1];
+                                const uint32_t r0 = (q & 1 ? c.y : c.x) >> (8 * half), r1 = (q & 1 ? c.w : c.z) >> (8 * half);
+#pragma unroll
+                                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                                    for (int part = PARTS - 1; part >= 0; --part) {
+                                        const uint4 v = xv[n][q][part];
+                                        mma_f16(acc[r][n], r0 & 0x000f000fu, r1 & 0x000f000fu, r0 & 0x00f000f0u, r1 & 0x00f000f0u, half ? v.z : v.x, half ? v.w : v.y);
+                                    }
+                            }
+                        if ((q + 1) % (GROUP / 32) == 0) {
+                            const int i = q / (GROUP / 32);
+#pragma unroll
+                            for (int r = 0; r < RT; ++r) {
+                                const uint32_t mm = m[d][r][i];
+                                const float s0 = __uint_as_float((mm << 16) & 0xfff00000u), s1 = __uint_as_float(mm & 0xfff00000u);
+                                const float z0 = (float)(mm & 15u), z1 = (float)((mm >> 16) & 15u);
+#pragma unroll
+                                for (int n = 0; n < NT; ++n) {
+                                    y[r][n].x = fmaf(s0, fmaf(z0, sx[n][i].x, acc[r][n][0]), y[r][n].x);
+                                    y[r][n].y = fmaf(s0, fmaf(z0, sx[n][i].y, acc[r][n][1]), y[r][n].y);
+                                    y[r][n].z = fmaf(s1, fmaf(z1, sx[n][i].x, acc[r][n][2]), y[r][n].z);
+                                    y[r][n].w = fmaf(s1, fmaf(z1, sx[n][i].y, acc[r][n][3]), y[r][n].w);
+                                }
+                            }
+                        }
+                    }
+                }
+                ask(d);
+#pragma unroll
+                for (int r = 0; r < RT; ++r) {
+                    if (j + r >= n_tiles) break;
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        float4* to = red + (((j + r) * p.ki + share) * NT + n) * 32 + lane;
+                        float4 v = make_float4(y[r][n].x * by[n].x, y[r][n].y * by[n].y, y[r][n].z * by[n].x, y[r][n].w * by[n].y);
+                        if (b >= c0 + p.ki) { const float4 o = *to; v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w; }
+                        *to = v;
+                    }
+                }
+            }
+        }
+    }
+
+    // the sums of all shares of K, in their order; a warp takes a tile's (gated: a pair of tiles') eight rows of x at a time
+    if (p.cs > 1) cluster_sync();
+    else __syncthreads();
+    const int step = p.mode == MODE_SILU_MUL ? 2 : 1;
+    for (int i = warp * p.cs + rank; i < n_tiles / step * NT; i += warps * p.cs) {
+        const int n = i % NT, at = i / NT * step;
+        float4 sum[2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            sum[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (r >= step) break;
+            for (int o = 0; o < p.cs; ++o) {
+#pragma unroll 4
+                for (int k = 0; k < p.ki; ++k) {
+                    const float4* from = red + (((at + r) * p.ki + k) * NT + n) * 32 + lane;
+                    const float4 v = p.cs > 1 ? ld_peer(from, o) : *from;
+                    sum[r].x += v.x; sum[r].y += v.y; sum[r].z += v.z; sum[r].w += v.w;
+                }
+            }
+        }
+        const float a[4] = {sum[0].x, sum[0].y, sum[0].z, sum[0].w}, u[4] = {sum[1].x, sum[1].y, sum[1].z, sum[1].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int token = n * 8 + 2 * t + (e & 1), o = (cta_tile + at) / step * 16 + g + (e & 2 ? 8 : 0);
+            if (token >= p.M || o >= (step == 2 ? p.half : p.rows)) continue;
+            const size_t to = (size_t)token * p.ldo + o;
+            if (step == 2) sp_st_dt(p.out, p.out_dt, to, sp_gated(a[e], u[e], p.ga));
+            else if (p.mode == MODE_ACCUMULATE) ((float*)p.out)[to] += a[e];
+            else sp_st_dt(p.out, p.out_dt, to, a[e]);
+        }
+    }
+    if (p.cs > 1) cluster_sync();                                    // nobody leaves before its sums are read
+}
+
+constexpr int SMEM_LIMIT = 200 * 1024;
+
+// How a product is divided: CTAs of a cluster and warps of a CTA that share K, sets of such warps, tiles of a CTA. A warp's time
+// goes with the tiles it multiplies, 0.5 us each at 8 rows; a further block of columns costs it about one and a half, a
+// cluster's exchange two. 8 rows of x (us, as chosen / the next best): 4,096 x 4,096 7.1 / 7.5, 4,096 x 14,336 16.2 / 17.2,
+// 2,048 x 8,192 8.9 / 9.0, gated 2 x 14,336 x 4,096 19.5 / 20.5.
+void divide(Product& p) {
+    const int sms = sp_sm_count() > 0 ? sp_sm_count() : 148;
+    double best = 0;
+    Product c = p;
+    for (c.cs = 1; c.cs <= 8 && c.cs <= p.blocks; c.cs *= 2) {
+        const int mine = (p.blocks + c.cs - 1) / c.cs, phases = (mine + MOST_WARPS - 1) / MOST_WARPS;
+        c.ki = (mine + phases - 1) / phases;
+        c.tpc = (p.tiles * c.cs + sms - 1) / sms;
+        if (p.mode == MODE_SILU_MUL) c.tpc += c.tpc & 1;
+        c.sets = MOST_WARPS / c.ki < c.tpc ? MOST_WARPS / c.ki : c.tpc;
+        const double cost = (double)((c.tpc + c.sets - 1) / c.sets) * phases + 1.5 * phases + (c.cs > 1 ? 2.0 : 0.0);
+        if (best == 0 || cost < best) { best = cost; p = c; }
+    }
+}
+
+template <typename TX, int NT, int GROUP>
+int launch_gemv(const TX* x, Product p, cudaStream_t stream) {
+    constexpr int RT = 1, DEPTH = sizeof(TX) == 4 ? 2 : 3;          // (two tiles at a time: 18.5 us instead of 19.5 where K is short, slower elsewhere)
+    static SpPerDevice configured;
+    if (!configured.done()) {
+        cudaError_t e = cudaFuncSetAttribute(gemv_kernel<TX, NT, GROUP, RT, DEPTH>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT);
+        if (e != cudaSuccess) SP_FAIL("q4_gemv: cannot reserve %d bytes of shared memory: %s", SMEM_LIMIT, cudaGetErrorString(e));
+        configured.mark();
+    }
+    divide(p);
+    while (p.tpc > 2 && p.tpc * p.ki * NT * 512 > SMEM_LIMIT) p.tpc -= 2;
+    const dim3 grid((p.tiles + p.tpc - 1) / p.tpc * p.cs);
+    SP_CHECK_CALL("q4_gemv", sp_launch_cluster(gemv_kernel<TX, NT, GROUP, RT, DEPTH>, grid, dim3(p.sets * p.ki * 32), (size_t)(p.tpc * p.ki * NT * 512), stream, p.cs, x, p));
+    return 0;
+}
+
 template <typename TX>
-cudaError_t launch_gemv(const TX* x, const Product& p, cudaStream_t stream) {
-    const dim3 grid((p.tiles + 1) / 2 * p.cs), block(WARPS * 32);
-    const bool two = p.M > 8, g32 = p.group == 32;
-    if (two) return g32 ? sp_launch_cluster(gemv_kernel<TX, 2, true>, grid, block, 0, stream, p.cs, x, p)
-                        : sp_launch_cluster(gemv_kernel<TX, 2, false>, grid, block, 0, stream, p.cs, x, p);
-    return g32 ? sp_launch_cluster(gemv_kernel<TX, 1, true>, grid, block, 0, stream, p.cs, x, p)
-               : sp_launch_cluster(gemv_kernel<TX, 1, false>, grid, block, 0, stream, p.cs, x, p);
+int launch_gemv(const void* xp, const Product& p, int group, cudaStream_t stream) {
+    const TX* x = (const TX*)xp;
+    if (p.M > 8) return group == 32 ? launch_gemv<TX, 2, 32>(x, p, stream) : group == 64 ? launch_gemv<TX, 2, 64>(x, p, stream) : launch_gemv<TX, 2, 128>(x, p, stream);
+    return group == 32 ? launch_gemv<TX, 1, 32>(x, p, stream) : group == 64 ? launch_gemv<TX, 1, 64>(x, p, stream) : launch_gemv<TX, 1, 128>(x, p, stream);
 }
 
 int check_sizes(const char* what, int rows, int K, int group, int half, int block) {
@@ -319,9 +401,9 @@ SP_API int sp_q4_packed_rows(int rows, int half) { return half ? (half + 15) / 1
 SP_API int sp_q4_pack(const void* w, int dt, long long ldw, void* codes, void* meta, int rows, int K, int group, int half, cudaStream_t stream) {
     if (check_sizes("q4_pack", rows, K, group, half, 0)) return 1;
     if ((uintptr_t)codes & 15) SP_FAIL("q4_pack: the codes must start on a 16-byte boundary");
-    const int packed = sp_q4_packed_rows(rows, half), kblocks = (K + 63) / 64;
-    pack_kernel<<<dim3(packed, (kblocks * 8 + 127) / 128), 128, 0, stream>>>(w, dt, ldw, (uint32_t*)codes, (uint16_t*)meta, rows, K,
-                                                                             kblocks, group, RowMap{half, 0});
+    const int packed = sp_q4_packed_rows(rows, half), blocks = (K + BLOCK - 1) / BLOCK;
+    pack_kernel<<<dim3(packed, (blocks * 16 + 127) / 128), blocks < 8 ? (blocks * 16 + 31) / 32 * 32 : 128, 0, stream>>>(w, dt, ldw, (uint32_t*)codes, (uint16_t*)meta, rows, K,
+                                                                             blocks, group, RowMap{half, 0});
     SP_CHECK_LAUNCH("q4_pack");
     return 0;
 }
@@ -330,10 +412,10 @@ SP_API int sp_q4_pack(const void* w, int dt, long long ldw, void* codes, void* m
 SP_API int sp_q4_unpack(const void* codes, const void* meta, void* out, int dt, int rows, int K, int group, int half, int block, cudaStream_t stream) {
     if (check_sizes("q4_unpack", rows, K, group, half, block)) return 1;
     if ((uintptr_t)out & 15) SP_FAIL("q4_unpack: the output must start on a 16-byte boundary");
-    const int packed = sp_q4_packed_rows(rows, half), kblocks = (K + 63) / 64;
-    const dim3 grid(packed, (kblocks * 8 + 127) / 128);
-    if (dt == SP_DT_F32) unpack_kernel<<<grid, 128, 0, stream>>>((const uint32_t*)codes, (const uint16_t*)meta, (float*)out, rows, K, kblocks, group, RowMap{half, block});
-    else unpack_kernel<<<grid, 128, 0, stream>>>((const uint32_t*)codes, (const uint16_t*)meta, (__nv_bfloat16*)out, rows, K, kblocks, group, RowMap{half, block});
+    const int packed = sp_q4_packed_rows(rows, half), blocks = (K + BLOCK - 1) / BLOCK;
+    const dim3 grid(packed, (blocks * 16 + 127) / 128);
+    if (dt == SP_DT_F32) unpack_kernel<<<grid, 128, 0, stream>>>((const uint32_t*)codes, (const uint16_t*)meta, (float*)out, rows, K, blocks, group, RowMap{half, block});
+    else unpack_kernel<<<grid, 128, 0, stream>>>((const uint32_t*)codes, (const uint16_t*)meta, (__nv_bfloat16*)out, rows, K, blocks, group, RowMap{half, block});
     SP_CHECK_LAUNCH("q4_unpack");
     return 0;
 }
@@ -348,11 +430,8 @@ SP_API int sp_q4_gemv(const void* x, int x_dt, const void* codes, const void* me
     if (mode == MODE_SILU_MUL && act != SP_ACT_SILU && act != SP_ACT_GELU) SP_FAIL("q4_gemv: activation code %d is not built for gated rows", act);
     if (mode == MODE_ACCUMULATE && out_dt != SP_DT_F32) SP_FAIL("q4_gemv: accumulation needs a float32 output");
     if (((uintptr_t)x & 15) || (ldx * (x_dt == SP_DT_F32 ? 4 : 2)) % 16) SP_FAIL("q4_gemv: rows of x must start on 16-byte boundaries");
-    if (((uintptr_t)codes & 15) || ((uintptr_t)meta & 1)) SP_FAIL("q4_gemv: codes must start on a 16-byte boundary");
-    const int packed = sp_q4_packed_rows(rows, half), kblocks = (K + 63) / 64, tiles = packed / 16;
-    Product p{(const uint4*)codes, (const uint16_t*)meta, out, ldx, ldo, out_dt, M, rows, tiles, kblocks, K, group, mode, half, 1, SpGate{act, mult}};
-    const int sms = sp_sm_count() > 0 ? sp_sm_count() : 148, pairs = (tiles + 1) / 2;
-    while (p.cs < 8 && pairs * p.cs < 3 * sms && kblocks >= 4 * WARPS * p.cs) p.cs *= 2;
-    SP_CHECK_CALL("q4_gemv", x_dt == SP_DT_F32 ? launch_gemv((const float*)x, p, stream) : launch_gemv((const __nv_bfloat16*)x, p, stream));
-    return 0;
+    if (((uintptr_t)codes & 15) || ((uintptr_t)meta & 15)) SP_FAIL("q4_gemv: codes and scales must start on 16-byte boundaries");
+    const int packed = sp_q4_packed_rows(rows, half), blocks = (K + BLOCK - 1) / BLOCK;
+    const Product p{(const uint8_t*)codes, (const uint8_t*)meta, out, ldx, ldo, out_dt, M, rows, packed / 16, blocks, K, mode, half, 1, 1, 1, 1, SpGate{act, mult}};
+    return x_dt == SP_DT_F32 ? launch_gemv<float>(x, p, group, stream) : launch_gemv<__nv_bfloat16>(x, p, group, stream);
 }
