@@ -346,17 +346,22 @@ constexpr int SMEM_LIMIT = 200 * 1024;
 // goes with the tiles it multiplies, 0.5 us each at 8 rows; a further block of columns costs it about one and a half, a
 // cluster's exchange two. 8 rows of x (us, as chosen / the next best): 4,096 x 4,096 7.1 / 7.5, 4,096 x 14,336 16.2 / 17.2,
 // 2,048 x 8,192 8.9 / 9.0, gated 2 x 14,336 x 4,096 19.5 / 20.5.
-void divide(Product& p) {
+// (Clusters of 4 and 8 do not find room on every SM and took two rounds: 4,096 x 14,336 40 us.) ``sum_bytes``: a tile's and share's partial sums.
+void divide(Product& p, int sum_bytes) {
     const int sms = sp_sm_count() > 0 ? sp_sm_count() : 148;
     double best = 0;
     Product c = p;
-    for (c.cs = 1; c.cs <= 8 && c.cs <= p.blocks; c.cs *= 2) {
+    for (c.cs = 1; c.cs <= 2 && c.cs <= p.blocks; ++c.cs) {
         const int mine = (p.blocks + c.cs - 1) / c.cs, phases = (mine + MOST_WARPS - 1) / MOST_WARPS;
         c.ki = (mine + phases - 1) / phases;
-        c.tpc = (p.tiles * c.cs + sms - 1) / sms;
+        const int clusters = sms / c.cs;
+        c.tpc = (p.tiles + clusters - 1) / clusters;
         if (p.mode == MODE_SILU_MUL) c.tpc += c.tpc & 1;
+        const int fits = SMEM_LIMIT / (c.ki * sum_bytes) & ~1;
+        int rounds = 1;
+        if (c.tpc > fits) { rounds = (c.tpc + fits - 1) / fits; c.tpc = fits; }
         c.sets = MOST_WARPS / c.ki < c.tpc ? MOST_WARPS / c.ki : c.tpc;
-        const double cost = (double)((c.tpc + c.sets - 1) / c.sets) * phases + 1.5 * phases + (c.cs > 1 ? 2.0 : 0.0);
+        const double cost = rounds * ((double)((c.tpc + c.sets - 1) / c.sets) * phases + 1.5 * phases + (c.cs > 1 ? 2.0 : 0.0) + 4.0);
         if (best == 0 || cost < best) { best = cost; p = c; }
     }
 }
@@ -370,8 +375,7 @@ int launch_gemv(const TX* x, Product p, cudaStream_t stream) {
         if (e != cudaSuccess) SP_FAIL("q4_gemv: cannot reserve %d bytes of shared memory: %s", SMEM_LIMIT, cudaGetErrorString(e));
         configured.mark();
     }
-    divide(p);
-    while (p.tpc > 2 && p.tpc * p.ki * NT * 512 > SMEM_LIMIT) p.tpc -= 2;
+    divide(p, NT * 512);
     const dim3 grid((p.tiles + p.tpc - 1) / p.tpc * p.cs);
     SP_CHECK_CALL("q4_gemv", sp_launch_cluster(gemv_kernel<TX, NT, GROUP, RT, DEPTH>, grid, dim3(p.sets * p.ki * 32), (size_t)(p.tpc * p.ki * NT * 512), stream, p.cs, x, p));
     return 0;
