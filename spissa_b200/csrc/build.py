@@ -65,11 +65,13 @@ MODULES = {
     "mlstm": "mlstm_kernels.cu",
     "q4": "q4_kernels.cu",
     "kv4": "kv4_kernels.cu",
+    "kv4_attention": "kv4_attention.cu",
 }
 # headers that only these modules include
 OWN_HEADERS = {
     "q4_kernels.cu": ["q4.cuh"],
     "kv4_kernels.cu": ["q4.cuh", "kv4.cuh"],
+    "kv4_attention.cu": ["q4.cuh", "kv4.cuh"],
 }
 
 

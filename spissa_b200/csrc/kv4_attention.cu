@@ -1,0 +1,582 @@
+// Attention over a cache of four bits (kv4_kernels.cu states the layout, q4.cuh the format): one token of each sequence, or a
+// few, over all the keys that they see, the keys split over CTAs and joined.
+//
+// score = scale · q · k̂, softmax in 32 bits, out = Σ p v̂; query head h reads kv head h / (heads / kv heads); a token at position p
+// sees keys p − window + 1 .. p.
+//
+// The cache is read once per kv head and 8 NT columns, a column being a query head of a token. Codes are used as they lie: the
+// four bits in the lowest place of a half word ARE the float16 c · 2^-24, one place up 16 c · 2^-24, so an AND makes an operand
+// of mma.sync m16n8k16, with 16 keys (scores) or 16 columns of the values (output) as its rows and the query columns as
+// its columns: nothing is wasted on padding up to eight heads. Scales and zeros are applied to what is small:
+//   score  Σ_groups s (Σ q' c − z Σ q'), q' = q times a power of two that brings a head's largest entry to 2^14 (exact for
+//          bfloat16; float32 as two float16 parts, 22 bits);
+//   output Σ_keys (p s) c − Σ_keys (p s) z: p s is rounded to float16 (2^-12 of itself; float32: two parts, 2^-23) under a
+//          reference that holds it below 2^15, so that the scale s of a key's group of values costs no rounding of the values.
+// The reference of a column follows its largest score, and the largest scale of the values, in steps: it moves only when a
+// score passes it by more than 2^8 or a scale passes the one it was made for; then the sums are multiplied by a power of two.
+//
+// A page of a kv head is one run of bytes and arrives by one bulk copy in a ring; four warps take 16 of its keys each and keep
+// sums of their own, joined at the end in the order of the warps, then of the chunks: results do not depend on timing.
+// A key or value that is not finite reaches the columns that see it and no others.
+#include "kv4.cuh"
+#include "async_copy.cuh"
+#include <cuda_fp16.h>
+
+SP_API const char* sp_kv4_attention_last_error() { return sp_error_text; }
+SP_DEFINE_RANGE_API(kv4_attention)
+
+namespace {
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr int WARPS = 4;
+constexpr int STAGES = 4;
+constexpr float STEP = 8.0f;                // how far a score may pass the reference, log2
+
+struct Args {
+    const void* q;                 // [T][nh * hd]
+    void* out;                     // the same shape
+    const uint8_t* pool;
+    const int* seq_start;          // [n_seqs + 1]; null: one token each
+    const int* positions;          // [T]
+    const int* seq_row;
+    const int* page_table;
+    const float* sink;             // [nh] or null
+    float* part;                   // [T * nh][n_chunks][hd], then [T * nh][n_chunks] (reference, sum); unused with one chunk
+    int* status;
+    int max_pages, nh, nkv, window, chunk_pages, n_chunks, T;
+    float scale;
+    SpRange rg;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t v) {          // of an 8 x 8 matrix of half words spread over the warp
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+__device__ __forceinline__ uint32_t half2_of(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *(const uint32_t*)&h;
+}
+__device__ __forceinline__ uint4 lds16(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+    return v;
+}
+// N words from shared memory, and N half words (as words of two)
+template <int N> __device__ __forceinline__ void lds_words(uint32_t at, uint32_t (&w)[N]) {
+    if constexpr (N == 4) asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at));
+    else if constexpr (N == 2) asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(at));
+    else
+#pragma unroll
+        for (int i = 0; i < N; ++i) asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[i]) : "r"(at + 4 * i));
+}
+template <int N> __device__ __forceinline__ void lds_halves(uint32_t at, uint32_t (&w)[(N + 1) / 2]) {
+    if constexpr (N == 4) asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(at));
+    else if constexpr (N == 2) asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[0]) : "r"(at));
+    else {
+#pragma unroll
+        for (int i = 0; i < (N + 1) / 2; ++i) w[i] = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            uint16_t h;
+            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(at + 2 * i));
+            w[i / 2] |= (uint32_t)h << (16 * (i & 1));
+        }
+    }
+}
+__device__ __forceinline__ float finite_or_nan(float v) { return fabsf(v) < INFINITY ? v : __int_as_float(0x7fc00000); }
+__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&v)[8]) {
+    const uint4 w = *(const uint4*)p;
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { v[2 * i] = finite_or_nan(__uint_as_float(u[i] << 16)); v[2 * i + 1] = finite_or_nan(__uint_as_float(u[i] & 0xffff0000u)); }
+}
+__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
+    const float4 a = *(const float4*)p, b = *(const float4*)(p + 4);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = finite_or_nan(v[i]);
+}
+
+// scale (group i of a row's half words) and zero as numbers; the zero through the place of ones of 2^23
+__device__ __forceinline__ float scale_at(const uint32_t* m, int i) {
+    return __uint_as_float(i & 1 ? m[i >> 1] & 0xfff00000u : (m[i >> 1] << 16) & 0xfff00000u);
+}
+__device__ __forceinline__ float zero_at(const uint32_t* m, int i) {
+    return __uint_as_float(((i & 1 ? m[i >> 1] >> 16 : m[i >> 1]) & 15u) | 0x4b000000u) - 8388608.0f;
+}
+
+template <typename TQ, int NG, int NT>
+__global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 2)
+attend_kernel(const Args a) {
+    constexpr int HD = 32 * NG, PARTS = sizeof(TQ) == 4 ? 2 : 1, COLS = 8 * NT, TILE = kv4_tile_bytes(HD), MW = (NG + 1) / 2;
+    constexpr bool Q_HELD = NT == 1 && PARTS == 1;                   // the queries' operands in registers, else in shared memory
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES];
+    __shared__ int failed;
+    __shared__ float ref_s[WARPS][COLS], sum_s[WARPS][COLS];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int seq = blockIdx.z, kvh = blockIdx.y % a.nkv, tile = blockIdx.y / a.nkv, chunk = blockIdx.x, G = a.nh / a.nkv;
+    const int tok0 = a.seq_start ? a.seq_start[seq] : seq, n_tok = a.seq_start ? a.seq_start[seq + 1] - tok0 : 1;
+    const int col0 = tile * COLS, n_cols = min(COLS, n_tok * G - col0);
+    if (n_cols <= 0) return;
+    const int first_pos = a.positions[tok0 + col0 / G], last_pos = a.positions[tok0 + (col0 + n_cols - 1) / G];        // of the tile's tokens
+    const int lowest = a.window ? max(0, first_pos + 1 - a.window) : 0;
+    const int page0 = lowest / KV4_PAGE + chunk * a.chunk_pages, page1 = min(page0 + a.chunk_pages, last_pos / KV4_PAGE + 1);
+    const int n_pages = max(0, page1 - page0), row = sp_checked_row(a.seq_row[seq], a.rg);
+    const int* table = a.page_table + (size_t)row * a.max_pages;
+    const uint32_t ring = smem_u32(smem), q_at = ring + STAGES * TILE;
+
+    if (threadIdx.x == 0) {
+        failed = 0;
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(smem_u32(&full[s]), 1);
+            mbar_init(smem_u32(&empty[s]), WARPS);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    __syncthreads();
+    auto fetch = [&](int i) {                                        // one thread
+        const int s = i % STAGES, page = sp_checked_page(table[sp_checked_entry(page0 + i, a.max_pages, a.rg)], a.rg);
+        mbar_expect_tx(smem_u32(&full[s]), TILE);
+        bulk_copy_g2s(ring + s * TILE, a.pool + ((size_t)page * a.nkv + kvh) * TILE, TILE, smem_u32(&full[s]));
+    };
+    if (threadIdx.x == 0)
+        for (int i = 0; i < min(STAGES, n_pages); ++i) fetch(i);
+
+    // The queries: lane (column g, dims 32 i + 8 t ..). Columns that are not there are zeros and see nothing.
+    uint32_t qh[Q_HELD ? NG : 1][4];
+    float unit[NT][2], qs[NT][NG][2];                                // of columns 2 t and 2 t + 1
+    int pos[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const int c = col0 + n * 8 + g, tok = min(c / G, n_tok - 1);
+        const bool there = n * 8 + g < n_cols;
+        const TQ* from = (const TQ*)a.q + ((size_t)(tok0 + tok) * a.nh + kvh * G + c % G) * HD + 8 * t;
+        float v[NG][8], top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+            load8(from + 32 * i, v[i]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                if (!there) v[i][e] = 0.0f;
+                top = fmaxf(top, fabsf(v[i][e]));
+            }
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int up = top > 0.0f ? min(94, max(-94, 141 - (int)(__float_as_uint(top) >> 23))) : 0;
+        const float by = __uint_as_float((uint32_t)(127 + up) << 23), back = __uint_as_float((uint32_t)(151 - up) << 23) * a.scale * LOG2E;
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+            float sum = 0.0f;
+            uint32_t h[PARTS][4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float lo = v[i][2 * j] * by, hi = v[i][2 * j + 1] * by, f = j & 1 ? 0.0625f : 1.0f;
+                sum += lo + hi;
+                h[0][j] = half2_of(lo * f, hi * f);
+                if (PARTS == 2) {
+                    const float2 first = __half22float2(*(const __half2*)&h[0][j]);
+                    h[PARTS - 1][j] = half2_of(lo * f - first.x, hi * f - first.y);
+                }
+            }
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            sum *= -5.9604644775390625e-8f;                          // −2^-24 Σ q', in the units of the codes' products
+            qs[n][i][0] = __shfl_sync(0xffffffffu, sum, 8 * t);
+            qs[n][i][1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4);
+            if (Q_HELD) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) qh[Q_HELD ? i : 0][j] = h[0][j];
+            } else if (warp == 0) {
+#pragma unroll
+                for (int part = 0; part < PARTS; ++part)
+                    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(q_at + (uint32_t)(((n * NG + i) * PARTS + part) * 32 + lane) * 16), "r"(h[part][0]), "r"(h[part][1]), "r"(h[part][2]), "r"(h[part][3]) : "memory");
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            unit[n][e] = __shfl_sync(0xffffffffu, back, 8 * t + 4 * e);
+            const int ce = n * 8 + 2 * t + e;
+            pos[n][e] = ce < n_cols ? a.positions[tok0 + (col0 + ce) / G] : -1;
+        }
+    }
+    if (!Q_HELD) __syncthreads();
+
+    float O[NT][NG][2][4], zs[NT][NG][2], sum[NT][2], ref[NT][2], top[NT][2];      // top: the score that the reference was made for
+    uint32_t poison[NT];
+    float s_top = 0.0f;                                              // the scale that the references were made for
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        poison[n] = 0;
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+            zs[n][i][0] = zs[n][i][1] = 0.0f;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) O[n][i][h][0] = O[n][i][h][1] = O[n][i][h][2] = O[n][i][h][3] = 0.0f;
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) { sum[n][e] = 0.0f; ref[n][e] = 0.0f; top[n][e] = -INFINITY; }
+    }
+
+    for (int it = 0; it < n_pages; ++it) {
+        const int s = it % STAGES, page_pos = (page0 + it) * KV4_PAGE;
+        // the stage that every warp had done with a page ago gets the next page
+        if (threadIdx.x == 0 && it >= 1 && it - 1 + STAGES < n_pages) {
+            if (mbar_wait_flag(smem_u32(&empty[(it - 1) % STAGES]), ((it - 1) / STAGES) & 1, a.status, 141, &failed)) fetch(it - 1 + STAGES);
+        }
+        __syncwarp();
+        mbar_wait_flag(smem_u32(&full[s]), (it / STAGES) & 1, a.status, 142, &failed);
+        const uint32_t at = ring + s * TILE;
+        const int r0 = warp * 16 + g;                                // rows of the page's keys as they lie: this lane's are r0 and r0 + 8
+        const int key = page_pos + warp * 16 + (g & 1) * 4 + (g >> 1);        // their positions: this and 8 on
+        const bool partly = page_pos + KV4_PAGE - 1 > first_pos || (a.window && page_pos < last_pos + 1 - a.window);
+
+        // scores of 16 keys: rows g and g + 8, columns 2 t and 2 t + 1
+        float x[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) x[n][0] = x[n][1] = x[n][2] = x[n][3] = 0.0f;
+        {
+            uint32_t k0[NG], k1[NG], m0[MW], m1[MW];
+            lds_words<NG>(at + r0 * (HD / 2) + t * (NG * 4), k0);
+            lds_words<NG>(at + (r0 + 8) * (HD / 2) + t * (NG * 4), k1);
+            lds_halves<NG>(at + kv4_k_meta(HD) + r0 * (NG * 2), m0);
+            lds_halves<NG>(at + kv4_k_meta(HD) + (r0 + 8) * (NG * 2), m1);
+#pragma unroll
+            for (int i = 0; i < NG; ++i) {
+                const float s0 = scale_at(m0, i), s1 = scale_at(m1, i), z0 = zero_at(m0, i), z1 = zero_at(m1, i);
+                const uint32_t u0 = k0[i], u1 = k1[i], w0 = u0 >> 8, w1 = u1 >> 8;
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int part = PARTS - 1; part >= 0; --part) {
+                        uint4 qv;
+                        if (Q_HELD) qv = make_uint4(qh[Q_HELD ? i : 0][0], qh[Q_HELD ? i : 0][1], qh[Q_HELD ? i : 0][2], qh[Q_HELD ? i : 0][3]);
+                        else qv = lds16(q_at + (uint32_t)(((n * NG + i) * PARTS + part) * 32 + lane) * 16);
+                        mma_f16(acc, u0 & 0x000f000fu, u1 & 0x000f000fu, u0 & 0x00f000f0u, u1 & 0x00f000f0u, qv.x, qv.y);
+                        mma_f16(acc, w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u, qv.z, qv.w);
+                    }
+                    x[n][0] = fmaf(s0, fmaf(z0, qs[n][i][0], acc[0]), x[n][0]);
+                    x[n][1] = fmaf(s0, fmaf(z0, qs[n][i][1], acc[1]), x[n][1]);
+                    x[n][2] = fmaf(s1, fmaf(z1, qs[n][i][0], acc[2]), x[n][2]);
+                    x[n][3] = fmaf(s1, fmaf(z1, qs[n][i][1], acc[3]), x[n][3]);
+                }
+            }
+        }
+        uint32_t m0[MW], m1[MW];                                     // the values' scales of the same two keys
+        {
+            const int p0 = warp * 16 + (g & 1) * 4 + (g >> 1);
+            lds_halves<NG>(at + kv4_v_meta(HD) + p0 * (NG * 2), m0);
+            lds_halves<NG>(at + kv4_v_meta(HD) + (p0 + 8) * (NG * 2), m1);
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                x[n][e] *= unit[n][e & 1];
+                if (partly) {
+                    const int p = pos[n][e & 1], j = key + (e & 2) * 4;
+                    if (j > p || (a.window && j <= p - a.window)) x[n][e] = -INFINITY;
+                }
+            }
+        if (partly) {                                                // what nobody sees may be anything
+#pragma unroll
+            for (int i = 0; i < MW; ++i) {
+                if (key > last_pos || key < lowest) m0[i] = 0;
+                if (key + 8 > last_pos || key + 8 < lowest) m1[i] = 0;
+            }
+        }
+        // do the references hold?
+        uint32_t most = 0;
+#pragma unroll
+        for (int i = 0; i < MW; ++i) most = __vmaxu2(most, __vmaxu2(m0[i], m1[i]));
+        most = max(most & 0xffffu, most >> 16);
+        bool moves = __uint_as_float((most & 0xfff0u) << 16) > s_top || (most & 0x7f80u) == 0x7f80u;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) moves |= x[n][e] > top[n][e & 1] + STEP;
+        if (__any_sync(0xffffffffu, moves)) {
+            // scales that are not numbers: noted for the columns that see their keys, and taken as zero
+#pragma unroll
+            for (int i = 0; i < NG; ++i) {
+                const int sh = 16 * (i & 1);
+                const bool bad0 = ((m0[i >> 1] >> sh) & 0x7f80u) == 0x7f80u, bad1 = ((m1[i >> 1] >> sh) & 0x7f80u) == 0x7f80u;
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        if ((bad0 && x[n][e] != -INFINITY) || (bad1 && x[n][2 + e] != -INFINITY)) poison[n] |= 1u << (2 * i + e);
+                if (bad0) m0[i >> 1] &= ~(0xffffu << sh);
+                if (bad1) m1[i >> 1] &= ~(0xffffu << sh);
+            }
+            most = 0;
+#pragma unroll
+            for (int i = 0; i < MW; ++i) most = __vmaxu2(most, __vmaxu2(m0[i], m1[i]));
+            most = max(most & 0xffffu, most >> 16);
+            const uint32_t all = __reduce_max_sync(0xffffffffu, most & 0xfff0u);
+            s_top = fmaxf(s_top, __uint_as_float(all << 16));
+            const float es = s_top > 0.0f ? (float)((int)(__float_as_uint(s_top) >> 23) - 126) : 0.0f;         // s_top < 2^es
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                float f[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float big = fmaxf(x[n][e], x[n][2 + e]);
+                    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 4));
+                    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 8));
+                    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 16));
+                    const bool had = top[n][e] != -INFINITY;
+                    if (big > top[n][e] + STEP) top[n][e] = big;
+                    const float was = ref[n][e];
+                    // p s <= 2^(STEP + top − ref + es) = 2^15; whole steps, so that the factors are powers of two
+                    ref[n][e] = top[n][e] != -INFINITY ? ceilf(top[n][e]) + es + STEP - 15.0f : 0.0f;
+                    f[e] = had ? ex2(was - ref[n][e]) : 1.0f;
+                    sum[n][e] *= f[e];
+                }
+#pragma unroll
+                for (int i = 0; i < NG; ++i) {
+                    zs[n][i][0] *= f[0];
+                    zs[n][i][1] *= f[1];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) { O[n][i][h][0] *= f[0]; O[n][i][h][1] *= f[1]; O[n][i][h][2] *= f[0]; O[n][i][h][3] *= f[1]; }
+                }
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[n][e] = ex2(x[n][e] - ref[n][e & 1]);
+            sum[n][0] += x[n][0] + x[n][2];
+            sum[n][1] += x[n][1] + x[n][3];
+        }
+        // the output of 16 keys
+        {
+            uint32_t v[4][MW];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int p = warp * 16 + 4 * k + t, sw = HD == 128 ? (p & 2) << 4 : 0;
+                lds_halves<NG>(at + kv4_v_codes(HD) + p * (HD / 2) + ((g * NG * 2) ^ sw), v[k]);
+            }
+#pragma unroll
+            for (int i = 0; i < NG; ++i) {
+                const float s0 = scale_at(m0, i), s1 = scale_at(m1, i), z0 = zero_at(m0, i), z1 = zero_at(m1, i);
+                const uint32_t u0 = __byte_perm(v[0][i >> 1], v[1][i >> 1], i & 1 ? 0x7632 : 0x5410), u1 = __byte_perm(v[2][i >> 1], v[3][i >> 1], i & 1 ? 0x7632 : 0x5410);
+                const uint32_t w0 = u0 >> 8, w1 = u1 >> 8;      // keys t, 4 + t and 8 + t, 12 + t side by side
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const float p0 = x[n][0] * s0, p1 = x[n][1] * s0, p2 = x[n][2] * s1, p3 = x[n][3] * s1;
+                    const uint32_t h0 = half2_of(p0, p1), h1 = half2_of(p2, p3), b0 = transposed(h0), b1 = transposed(h1);
+                    mma_f16(O[n][i][0], u0 & 0x000f000fu, u0 & 0x00f000f0u, u1 & 0x000f000fu, u1 & 0x00f000f0u, b0, b1);
+                    mma_f16(O[n][i][1], w0 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x000f000fu, w1 & 0x00f000f0u, b0, b1);
+                    // (the zeros are taken off with the same rounded numbers, so that a value of zero adds exactly nothing)
+                    float2 f0 = __half22float2(*(const __half2*)&h0), f1 = __half22float2(*(const __half2*)&h1);
+                    if (PARTS == 2) {
+                        const uint32_t l0 = half2_of(p0 - f0.x, p1 - f0.y), l1 = half2_of(p2 - f1.x, p3 - f1.y), c0 = transposed(l0), c1 = transposed(l1);
+                        mma_f16(O[n][i][0], u0 & 0x000f000fu, u0 & 0x00f000f0u, u1 & 0x000f000fu, u1 & 0x00f000f0u, c0, c1);
+                        mma_f16(O[n][i][1], w0 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x000f000fu, w1 & 0x00f000f0u, c0, c1);
+                        const float2 r0 = __half22float2(*(const __half2*)&l0), r1 = __half22float2(*(const __half2*)&l1);
+                        f0.x += r0.x; f0.y += r0.y; f1.x += r1.x; f1.y += r1.y;
+                    }
+                    zs[n][i][0] = fmaf(f0.x, z0, fmaf(f1.x, z1, zs[n][i][0]));
+                    zs[n][i][1] = fmaf(f0.y, z0, fmaf(f1.y, z1, zs[n][i][1]));
+                }
+            }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&empty[s]));
+    }
+
+    // each warp's sums over its lanes; then the warps', in their order, in shared memory (where the pages were)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int o = 4; o < 32; o *= 2) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                sum[n][e] += __shfl_xor_sync(0xffffffffu, sum[n][e], o);
+#pragma unroll
+                for (int i = 0; i < NG; ++i) zs[n][i][e] += __shfl_xor_sync(0xffffffffu, zs[n][i][e], o);
+            }
+            poison[n] |= __shfl_xor_sync(0xffffffffu, poison[n], o);
+        }
+        if (g == 0)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                ref_s[warp][n * 8 + 2 * t + e] = top[n][e] == -INFINITY && sum[n][e] == 0.0f ? -INFINITY : ref[n][e];
+                sum_s[warp][n * 8 + 2 * t + e] = sum[n][e];
+            }
+    }
+    __syncthreads();
+    float* acc = (float*)smem;                                       // [column][HD]
+    for (int w = 0; w < WARPS; ++w) {
+        if (warp == w) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int c = n * 8 + 2 * t + e;
+                    float big = ref_s[0][c];
+#pragma unroll
+                    for (int k = 1; k < WARPS; ++k) big = fmaxf(big, ref_s[k][c]);
+                    const float f = ref_s[w][c] == -INFINITY ? 0.0f : ex2(ref_s[w][c] - big);
+#pragma unroll
+                    for (int i = 0; i < NG; ++i)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            float2* to = (float2*)(acc + c * HD + 32 * i + 4 * g + 2 * h);
+                            float2 v = make_float2(fmaf(O[n][i][h][e], 16777216.0f, -zs[n][i][e]) * f, fmaf(O[n][i][h][2 + e], 1048576.0f, -zs[n][i][e]) * f);
+                            if (f == 0.0f) v = make_float2(0.0f, 0.0f);
+                            if (poison[n] >> (2 * i + e) & 1) v.x = v.y = __int_as_float(0x7fc00000);
+                            if (w > 0) { v.x += to->x; v.y += to->y; }
+                            *to = v;
+                        }
+                }
+        }
+        __syncthreads();
+    }
+    if (failed) return;
+    for (int c = warp; c < n_cols; c += WARPS) {
+        float big = ref_s[0][c], total = 0.0f;
+#pragma unroll
+        for (int k = 1; k < WARPS; ++k) big = fmaxf(big, ref_s[k][c]);
+#pragma unroll
+        for (int k = 0; k < WARPS; ++k) total += ref_s[k][c] == -INFINITY ? 0.0f : sum_s[k][c] * ex2(ref_s[k][c] - big);
+        const int tok = tok0 + (col0 + c) / G, head = kvh * G + (col0 + c) % G;
+        const size_t out_row = (size_t)tok * a.nh + head;
+        if (a.n_chunks > 1) {
+            float* part = a.part + (out_row * a.n_chunks + chunk) * HD;
+            for (int d = lane; d < HD; d += 32) part[d] = acc[c * HD + d];
+            if (lane == 0) ((float2*)(a.part + (size_t)a.T * a.nh * a.n_chunks * HD))[out_row * a.n_chunks + chunk] = make_float2(big, total);
+            continue;
+        }
+        float f = 1.0f;
+        if (a.sink) {
+            const float y = a.sink[head] * LOG2E, most = fmaxf(big, y);
+            f = big == -INFINITY ? 0.0f : ex2(big - most);
+            total = total * f + ex2(y - most);
+        }
+        const float inv = big == -INFINITY ? 0.0f : f / total;       // (no key seen: zeros)
+        for (int d = lane; d < HD; d += 32) {
+            const float v = big == -INFINITY ? 0.0f : acc[c * HD + d] * inv;
+            sp_st((TQ*)a.out, out_row * HD + d, v);
+        }
+    }
+}
+
+// The chunks' sums of a row (a token's head), in their order: a warp a row.
+template <typename TQ>
+__global__ void __launch_bounds__(128)
+join_kernel(const Args a, int hd) {
+    sp_wait_for_predecessor();
+    const int lane = threadIdx.x & 31;
+    const size_t rows = (size_t)a.T * a.nh, row = (size_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+    if (row >= rows) return;
+    const float* part = a.part + row * a.n_chunks * hd;
+    const float2* heads = (const float2*)(a.part + rows * a.n_chunks * hd) + row * a.n_chunks;
+    float big = -INFINITY;
+    for (int c = lane; c < a.n_chunks; c += 32) big = fmaxf(big, sp_ld_written(heads + c).x);
+    big = sp_warp_max(big);
+    float sum = 0.0f;
+    for (int c = lane; c < a.n_chunks; c += 32) {
+        const float2 h = sp_ld_written(heads + c);
+        if (h.x != -INFINITY) sum += h.y * ex2(h.x - big);
+    }
+    float f = 1.0f, total = sp_warp_sum(sum);
+    if (a.sink) {
+        const float y = a.sink[row % a.nh] * LOG2E, most = fmaxf(big, y);
+        f = big == -INFINITY ? 0.0f : ex2(big - most);
+        total = total * f + ex2(y - most);
+    }
+    float v[KV4_MAX_HD / 32] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int c0 = 0; c0 < a.n_chunks; c0 += 32) {
+        const float2 h = c0 + lane < a.n_chunks ? sp_ld_written(heads + c0 + lane) : make_float2(-INFINITY, 0.0f);
+        const float mine = h.x == -INFINITY ? 0.0f : ex2(h.x - big);
+        for (int c = 0; c < min(32, a.n_chunks - c0); ++c) {
+            const float w = __shfl_sync(0xffffffffu, mine, c);
+            if (w == 0.0f) continue;                                 // a chunk without a key that the row sees
+#pragma unroll
+            for (int k = 0; k < KV4_MAX_HD / 32; ++k)
+                if (32 * k < hd) v[k] = fmaf(w, sp_ld_written(part + (size_t)(c0 + c) * hd + 32 * k + lane), v[k]);
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < KV4_MAX_HD / 32; ++k)
+        if (32 * k < hd) sp_st((TQ*)a.out, row * hd + 32 * k + lane, big == -INFINITY ? 0.0f : v[k] * f / total);
+}
+
+template <typename TQ, int NG, int NT>
+int launch(const Args& a, int n_seqs, int tiles, cudaStream_t stream) {
+    constexpr int PARTS = sizeof(TQ) == 4 ? 2 : 1, RING = STAGES * kv4_tile_bytes(32 * NG), ACC = 8 * NT * 32 * NG * 4;
+    constexpr int SMEM = (RING > ACC ? RING : ACC) + (NT == 1 && PARTS == 1 ? 0 : NT * NG * PARTS * 512);
+    static_assert(RING >= ACC, "the joined sums lie where the pages were");
+    static SpPerDevice configured;
+    if (!configured.done()) {
+        cudaError_t e = cudaFuncSetAttribute(attend_kernel<TQ, NG, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+        if (e != cudaSuccess) SP_FAIL("kv4_attention: cannot reserve %d bytes of shared memory: %s", SMEM, cudaGetErrorString(e));
+        configured.mark();
+    }
+    attend_kernel<TQ, NG, NT><<<dim3(a.n_chunks, a.nkv * tiles, n_seqs), WARPS * 32, SMEM, stream>>>(a);
+    SP_CHECK_LAUNCH("kv4_attention");
+    if (a.n_chunks > 1)
+        SP_CHECK_CALL("kv4_attention", sp_launch_dependent(join_kernel<TQ>, dim3((unsigned)(((size_t)a.T * a.nh + 3) / 4)), dim3(128), 0, stream, a, 32 * NG));
+    return 0;
+}
+
+template <typename TQ, int NG>
+int launch(const Args& a, int n_seqs, int nt, int max_new, cudaStream_t stream) {
+    const int G = a.nh / a.nkv, tiles = (max_new * G + 8 * nt - 1) / (8 * nt);
+    if ((long long)a.nkv * tiles > 65535 || n_seqs > 65535) SP_FAIL("kv4_attention: %d sequences of %d tokens, %d kv heads", n_seqs, max_new, a.nkv);
+    if (nt == 4) return launch<TQ, NG, 4>(a, n_seqs, tiles, stream);
+    if (nt == 2) return launch<TQ, NG, 2>(a, n_seqs, tiles, stream);
+    return launch<TQ, NG, 1>(a, n_seqs, tiles, stream);
+}
+
+template <typename TQ>
+int launch(const Args& a, int n_seqs, int nt, int max_new, int hd, cudaStream_t stream) {
+    switch (hd) {
+        case 32: return launch<TQ, 1>(a, n_seqs, nt, max_new, stream);
+        case 64: return launch<TQ, 2>(a, n_seqs, nt, max_new, stream);
+        case 96: return launch<TQ, 3>(a, n_seqs, nt, max_new, stream);
+        default: return launch<TQ, 4>(a, n_seqs, nt, max_new, stream);
+    }
+}
+
+}  // namespace
+
+// Floats of scratch that a call needs.
+SP_API long long sp_kv4_attend_scratch(int T, int nh, int hd, int n_chunks) { return n_chunks > 1 ? (long long)T * nh * n_chunks * (hd + 2) : 0; }
+
+// out [T, nh·hd] for queries q of the same shape and type (bfloat16 or float32). ``seq_start`` [n_seqs + 1], null: one token a
+// sequence. ``max_new``: the most tokens of a sequence. ``nt``: 8 nt columns a CTA (1, 2 or 4). ``chunk_pages``, ``n_chunks``:
+// the split of the keys, from the first that a CTA's tokens see.
+SP_API int sp_kv4_attend(const void* q, void* out, int dt, const void* pool, const int* seq_start, const int* positions, const int* seq_row,
+                         const int* page_table, int max_pages, int page_size, int T, int n_seqs, int max_new, int nh, int nkv, int hd,
+                         int window, float scale, const float* sink, int nt, int chunk_pages, int n_chunks, float* scratch,
+                         long long scratch_floats, int* status, cudaStream_t stream) {
+    if (T <= 0 || n_seqs <= 0) return 0;
+    if (hd <= 0 || hd % 32 || hd > KV4_MAX_HD) SP_FAIL("kv4_attention: head sizes 32, 64, 96 and 128, got %d", hd);
+    if (page_size != KV4_PAGE) SP_FAIL("kv4_attention: pages of %d positions, got %d", KV4_PAGE, page_size);
+    if (nkv <= 0 || nh <= 0 || nh % nkv) SP_FAIL("kv4_attention: %d heads are no multiple of %d kv heads", nh, nkv);
+    if (nt != 1 && nt != 2 && nt != 4) SP_FAIL("kv4_attention: 8, 16 or 32 columns a CTA, got 8 x %d", nt);
+    if (window < 0 || max_new <= 0 || (!seq_start && (max_new != 1 || T != n_seqs))) SP_FAIL("kv4_attention: window %d, %d tokens of %d sequences, at most %d of one", window, T, n_seqs, max_new);
+    if (chunk_pages <= 0 || n_chunks <= 0 || n_chunks > 65535) SP_FAIL("kv4_attention: %d chunks of %d pages", n_chunks, chunk_pages);
+    if (((uintptr_t)q & 15) || ((uintptr_t)pool & 15)) SP_FAIL("kv4_attention: queries and pages must start on 16-byte boundaries");
+    if (sp_kv4_attend_scratch(T, nh, hd, n_chunks) > scratch_floats) SP_FAIL("kv4_attention: %lld floats of scratch are needed, got %lld", sp_kv4_attend_scratch(T, nh, hd, n_chunks), scratch_floats);
+    const Args a{q, out, (const uint8_t*)pool, seq_start, positions, seq_row, page_table, sink, scratch, status,
+                 max_pages, nh, nkv, window, chunk_pages, n_chunks, T, scale, sp_range_host};
+    return dt == SP_DT_F32 ? launch<float>(a, n_seqs, nt, max_new, hd, stream) : launch<__nv_bfloat16>(a, n_seqs, nt, max_new, hd, stream);
+}

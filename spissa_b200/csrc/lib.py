@@ -47,6 +47,9 @@ def load(module: str) -> ctypes.CDLL:
             # declared once: plain integers pass, without an object made for each of a call's arguments
             lib.sp_q4_gemv.argtypes = [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_longlong,
                                        c_longlong, c_int, c_int, c_float, c_void_p]
+        if module == "kv4_attention":
+            lib.sp_kv4_attend.argtypes = [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p] + [c_int] * 9 + \
+                [c_float, c_void_p, c_int, c_int, c_int, c_void_p, c_longlong, c_void_p, c_void_p]
         if module == "seqmix":
             lib.sp_retention_chunked_scratch_floats.restype = c_longlong
         if module == "mlstm":
@@ -1918,3 +1921,47 @@ def kv4_unpack_pages(pool, meta, k_out, v_out, table, step, window, nkv, hd) -> 
         c_void_p(_ptr(step.seq_len)), c_void_p(_ptr(step.seq_start)), c_void_p(_ptr(meta.positions)), int(window or 0),
         c_void_p(_ptr(meta.seq_slot)), c_void_p(_ptr(pt)), pt.shape[1], meta.page_size, int(step.n_seqs), k_out.shape[0], int(nkv), int(hd),
         c_void_p(_stream())))
+
+
+def kv4_attend_plan(n_seqs: int, nkv: int, cols: int, pages: int) -> tuple:
+    """(tiles of eight columns a CTA takes, pages per chunk, chunks) for ``kv4_attend``: ``cols`` query columns (heads of a kv head
+    times tokens) of the sequence with the most, ``pages`` of keys that the longest sequence's tokens see."""
+    nt = 1 if cols <= 8 else 2 if cols <= 16 else 4
+    base = n_seqs * nkv * -(-cols // (8 * nt))
+    n_chunks = min(max(1, -(-pages // 2)), max(1, round((592 if nt == 1 else 296) / base)))
+    chunk_pages = -(-pages // n_chunks)
+    return nt, chunk_pages, -(-pages // chunk_pages)
+
+
+def kv4_attend(q, pool, out, meta, seq_start, n_seqs: int, max_new: int, longest: int, nh, nkv, hd, window, scale, sink=None, plan=None) -> None:
+    """Attention of the step's tokens over the four-bit pages, every key read once per kv head and tile of query columns.
+    ``seq_start`` [n_seqs + 1] int32, or None where every sequence brings one token; ``max_new``: the most tokens of a sequence;
+    ``longest``: the keys that the longest sequence may have (it shapes the split of the keys)."""
+    T = q.shape[0]
+    if q.dtype not in _DT or tuple(q.shape) != (T, nh * hd) or out.shape != q.shape or out.dtype != q.dtype or nh % nkv:
+        raise KernelError(f"kv4_attend: queries and output are [tokens, {nh} x {hd}] of one type, of heads in equal groups")
+    if sink is not None and (sink.dtype != torch.float32 or sink.numel() != nh):
+        raise KernelError("kv4_attend: the sinks are one float32 per query head")
+    _kv4_check("kv4_attend", pool, meta, T, nkv, hd, q, out, seq_start, sink)
+    if seq_start is not None and (seq_start.dtype != torch.int32 or seq_start.numel() < n_seqs + 1):
+        raise KernelError("kv4_attend: the sequences' first tokens are int32, one more than sequences")
+    lib = load("kv4_attention")
+    pt = meta.page_table
+    window = int(window or 0)
+    pages = -(-longest // 64)
+    if window:
+        pages = min(pages, (window + max_new - 2) // 64 + 2)
+    nt, chunk_pages, n_chunks = plan or kv4_attend_plan(n_seqs, nkv, max_new * (nh // nkv), max(1, pages))
+    need = T * nh * n_chunks * (hd + 2) if n_chunks > 1 else 0
+    scratch = torch.empty(need, dtype=torch.float32, device=q.device) if need else None
+    _declare_bounds("kv4_attention", lib, _pool_pages(meta, pool), _table_rows(meta, pt), q.device)
+    rc = lib.sp_kv4_attend(
+        q.data_ptr(), out.data_ptr(), dt_code(q), pool.data_ptr(), seq_start.data_ptr() if seq_start is not None else None,
+        meta.positions.data_ptr(), meta.seq_slot.data_ptr(), pt.data_ptr(), pt.shape[1], meta.page_size, T, n_seqs, max_new, nh, nkv, hd, window,
+        scale, sink.data_ptr() if sink is not None else None, nt, chunk_pages, n_chunks, scratch.data_ptr() if need else None, need,
+        status_word(q.device).data_ptr(), _stream())
+    if rc:
+        _check("kv4_attention", rc)
+    if n_chunks > 1:
+        global launches
+        launches += 1        # two kernels: the chunks and their joining

@@ -44,6 +44,7 @@ def length_bucket(max_len: int, page_size: int) -> int:
 
 
 FLASH_TC_TOKENS = 256      # bfloat16 prompt steps of at least so many tokens take the tcgen05 attention
+SPLIT4_COLUMNS = 256       # prompt steps of up to so many query columns (tokens x heads of a kv head) read a four-bit cache as it lies
 TILED_TOKENS = 32          # 32-bit prompt steps of at least so many tokens take the attention kernel of 64-query tiles
 
 
@@ -215,6 +216,13 @@ def attend_four_bits(q, step, cache, nh, nkv, hd, window, scale, sink=None):
     T = q.shape[0]
     if q.dtype not in (torch.bfloat16, torch.float32) or tuple(q.shape) != (T, nh * hd) or nh % nkv:
         raise K.KernelError(f"attention: queries are [tokens, {nh} x {hd}], bfloat16 or float32, of heads in equal groups")
+    if step.all_single or step.max_new * (nh // nkv) <= SPLIT4_COLUMNS:
+        out = torch.empty_like(q)
+        # (a decode step by its length's bucket, as below: run directly and replayed from a graph it adds up in the same order)
+        longest = length_bucket(step.max_len, cache.page_size) if step.all_single else step.max_len
+        K.kv4_attend(q, cache.k_pool, out, cache, None if step.all_single else step.seq_start, step.n_seqs, step.max_new, longest, nh, nkv, hd,
+                     window, scale, sink)
+        return out
     lens = step.host.get("seq_len") or step.seq_len.tolist()
     n_pages = sum(-(-n // cache.page_size) for n in lens)
     k = torch.empty(n_pages, nkv, cache.page_size, hd, dtype=q.dtype, device=q.device)

@@ -237,13 +237,16 @@ def attention_case(nh, nkv, hd, dtype, new, before, window, seed, sink=False):
     q = numbers(sum(new), nh, hd, seed=seed + 99, spread=0.2, dtype=dtype)
     sinks = numbers(1, nh, seed=seed + 7, spread=0.1)[0].contiguous() if sink else None
     scale = 1.0 / math.sqrt(hd)
-    outs, mags, at = [], [], 0
+    outs, mags, spans, at = [], [], [], 0
     for (k, v), n, b in zip(kv, new, before):
         kh, vh = Q.q4(k, 32), Q.q4(v, 32)
         outs.append(Q.attention(q[at:at + n], kh, vh, b, scale, window, sinks))
         mags.append(Q.attention(q[at:at + n], kh, vh.abs(), b, scale, window, sinks))
+        span = v.double().reshape(*v.shape[:2], -1, 32)              # 15 s of every group: its range and up to an eighth more
+        span = 1.125 * (span.amax(-1).clamp(min=0) - span.amin(-1).clamp(max=0)).repeat_interleave(32, -1)
+        spans.append((b + n) * Q.attention(q[at:at + n], kh, span, b, scale, window, sinks))
         at += n
-    return meta, kv, q, sinks, torch.cat(outs).reshape(sum(new), -1), torch.cat(mags).reshape(sum(new), -1)
+    return meta, kv, q, sinks, *(torch.cat(x).reshape(sum(new), -1) for x in (outs, mags, spans))
 
 
 def run_attention(meta, pool, q, nh, nkv, hd, window, sinks, new, before):
@@ -268,13 +271,15 @@ CASES = [([1], [0]), ([1], [63]), ([1, 1, 1], [64, 0, 700]), ([1], [2500]), ([2,
 def test_attention(case, nh, nkv, hd, dtype):
     new, before = CASES[case]
     for window, sink in ((None, False), (70, True)):
-        meta, kv, q, sinks, want, mag = attention_case(nh, nkv, hd, dtype, new, before, window, 10 * case + hd, sink)
+        meta, kv, q, sinks, want, mag, span = attention_case(nh, nkv, hd, dtype, new, before, window, 10 * case + hd, sink)
         pool = fill(meta, kv, nkv, hd)
         out = run_attention(meta, pool, q, nh, nkv, hd, window, sinks, new, before)
         assert out.dtype == dtype and out.shape == want.shape
         # scores: sums of hd products and a scale, off by (hd + 8) 2^-23 of their terms' sizes, which are below 64 here, so each
-        # probability by that (e^x − 1 is near x); bfloat16: probabilities and outputs rounded on top, 2^-8 each
+        # probability by that (e^x − 1 is near x); bfloat16: probabilities and outputs rounded on top, 2^-8 each. A value enters as
+        # p s c − p s z: two sums over the n keys of terms up to 15 s p, whose partial sums are cut to 24 bits at every step, so
+        # that each is off by at most n 2^-23 Σ 15 s p, also where c = z leaves nothing of the value itself (``span``: n Σ 15 s p)
         eps = (hd + 8) * 2.0 ** -23 * 64
-        tol = 2 * eps * mag + (2.0 ** -8 * mag + 2.0 ** -8 * want.abs() if dtype == BF else 0)
+        tol = 2 * eps * mag + 2 * 2.0 ** -23 * span + (2.0 ** -8 * mag + 2.0 ** -8 * want.abs() if dtype == BF else 0)
         assert bool(((out.cpu().double() - want).abs() <= tol).all()), float(((out.cpu().double() - want).abs() / tol).max())
         assert torch.equal(out, run_attention(meta, pool, q, nh, nkv, hd, window, sinks, new, before))
