@@ -12,6 +12,8 @@
 //          bfloat16; float32 as two float16 parts, 22 bits);
 //   output Σ_keys (p s) c − Σ_keys (p s) z: p s is rounded to float16 (2^-12 of itself; float32: two parts, 2^-23) under a
 //          reference that holds it below 2^15, so that the scale s of a key's group of values costs no rounding of the values.
+// With float32 queries the operands are c − z itself (1024 + c less 1024 + z), and a page's sums are added in 32 bits: tensor
+// cores cut partial sums to 24 bits, and sums of p s c are many times those of p s (c − z).
 // The reference of a column follows its largest score, and the largest scale of the values, in steps: it moves only when a
 // score passes it by more than 2^8 or a scale passes the one it was made for; then the sums are multiplied by a power of two.
 //
@@ -177,7 +179,7 @@ attend_kernel(const Args a) {
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         const int up = top > 0.0f ? min(94, max(-94, 141 - (int)(__float_as_uint(top) >> 23))) : 0;
-        const float by = __uint_as_float((uint32_t)(127 + up) << 23), back = __uint_as_float((uint32_t)(151 - up) << 23) * a.scale * LOG2E;
+        const float by = __uint_as_float((uint32_t)(127 + up) << 23), back = __uint_as_float((uint32_t)((PARTS == 2 ? 127 : 151) - up) << 23) * a.scale * LOG2E;
 #pragma unroll
         for (int i = 0; i < NG; ++i) {
             float sum = 0.0f;
@@ -258,6 +260,12 @@ attend_kernel(const Args a) {
             for (int i = 0; i < NG; ++i) {
                 const float s0 = scale_at(m0, i), s1 = scale_at(m1, i), z0 = zero_at(m0, i), z1 = zero_at(m1, i);
                 const uint32_t u0 = k0[i], u1 = k1[i], w0 = u0 >> 8, w1 = u1 >> 8;
+                uint32_t c[8] = {u0 & 0x000f000fu, u1 & 0x000f000fu, u0 & 0x00f000f0u, u1 & 0x00f000f0u, w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u};
+                if (PARTS == 2) {
+                    const uint32_t y0 = ((m0[i >> 1] >> (16 * (i & 1))) & 15u) * 0x10001u, y1 = ((m1[i >> 1] >> (16 * (i & 1))) & 15u) * 0x10001u;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) c[j] = q4_less(c[j], (j & 1 ? y1 : y0) << (j & 2 ? 4 : 0));
+                }
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     float acc[4] = {0.f, 0.f, 0.f, 0.f};
@@ -266,8 +274,15 @@ attend_kernel(const Args a) {
                         uint4 qv;
                         if (Q_HELD) qv = make_uint4(qh[Q_HELD ? i : 0][0], qh[Q_HELD ? i : 0][1], qh[Q_HELD ? i : 0][2], qh[Q_HELD ? i : 0][3]);
                         else qv = lds16(q_at + (uint32_t)(((n * NG + i) * PARTS + part) * 32 + lane) * 16);
-                        mma_f16(acc, u0 & 0x000f000fu, u1 & 0x000f000fu, u0 & 0x00f000f0u, u1 & 0x00f000f0u, qv.x, qv.y);
-                        mma_f16(acc, w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u, qv.z, qv.w);
+                        mma_f16(acc, c[0], c[1], c[2], c[3], qv.x, qv.y);
+                        mma_f16(acc, c[4], c[5], c[6], c[7], qv.z, qv.w);
+                    }
+                    if (PARTS == 2) {
+                        x[n][0] = fmaf(s0, acc[0], x[n][0]);
+                        x[n][1] = fmaf(s0, acc[1], x[n][1]);
+                        x[n][2] = fmaf(s1, acc[2], x[n][2]);
+                        x[n][3] = fmaf(s1, acc[3], x[n][3]);
+                        continue;
                     }
                     x[n][0] = fmaf(s0, fmaf(z0, qs[n][i][0], acc[0]), x[n][0]);
                     x[n][1] = fmaf(s0, fmaf(z0, qs[n][i][1], acc[1]), x[n][1]);
@@ -365,32 +380,46 @@ attend_kernel(const Args a) {
         }
         // the output of 16 keys
         {
-            uint32_t v[4][MW];
+            uint32_t v[4][MW], mz[PARTS == 2 ? 4 : 1][MW];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const int p = warp * 16 + 4 * k + t, sw = HD == 128 ? (p & 2) << 4 : 0;
                 lds_halves<NG>(at + kv4_v_codes(HD) + p * (HD / 2) + ((g * NG * 2) ^ sw), v[k]);
+                if (PARTS == 2) lds_halves<NG>(at + kv4_v_meta(HD) + p * (NG * 2), mz[PARTS == 2 ? k : 0]);
             }
 #pragma unroll
             for (int i = 0; i < NG; ++i) {
                 const float s0 = scale_at(m0, i), s1 = scale_at(m1, i), z0 = zero_at(m0, i), z1 = zero_at(m1, i);
                 const uint32_t u0 = __byte_perm(v[0][i >> 1], v[1][i >> 1], i & 1 ? 0x7632 : 0x5410), u1 = __byte_perm(v[2][i >> 1], v[3][i >> 1], i & 1 ? 0x7632 : 0x5410);
                 const uint32_t w0 = u0 >> 8, w1 = u1 >> 8;      // keys t, 4 + t and 8 + t, 12 + t side by side
+                uint32_t c[8] = {u0 & 0x000f000fu, u0 & 0x00f000f0u, u1 & 0x000f000fu, u1 & 0x00f000f0u, w0 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x000f000fu, w1 & 0x00f000f0u};
+                if (PARTS == 2) {
+                    const uint32_t y0 = __byte_perm(mz[0][i >> 1], mz[PARTS == 2 ? 1 : 0][i >> 1], i & 1 ? 0x7632 : 0x5410) & 0x000f000fu;
+                    const uint32_t y1 = __byte_perm(mz[PARTS == 2 ? 2 : 0][i >> 1], mz[PARTS == 2 ? 3 : 0][i >> 1], i & 1 ? 0x7632 : 0x5410) & 0x000f000fu;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) c[j] = q4_less(c[j], (j & 2 ? y1 : y0) << (j & 1 ? 4 : 0));
+                }
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     const float p0 = x[n][0] * s0, p1 = x[n][1] * s0, p2 = x[n][2] * s1, p3 = x[n][3] * s1;
                     const uint32_t h0 = half2_of(p0, p1), h1 = half2_of(p2, p3), b0 = transposed(h0), b1 = transposed(h1);
-                    mma_f16(O[n][i][0], u0 & 0x000f000fu, u0 & 0x00f000f0u, u1 & 0x000f000fu, u1 & 0x00f000f0u, b0, b1);
-                    mma_f16(O[n][i][1], w0 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x000f000fu, w1 & 0x00f000f0u, b0, b1);
-                    // (the zeros are taken off with the same rounded numbers, so that a value of zero adds exactly nothing)
-                    float2 f0 = __half22float2(*(const __half2*)&h0), f1 = __half22float2(*(const __half2*)&h1);
+                    const float2 f0 = __half22float2(*(const __half2*)&h0), f1 = __half22float2(*(const __half2*)&h1);
                     if (PARTS == 2) {
-                        const uint32_t l0 = half2_of(p0 - f0.x, p1 - f0.y), l1 = half2_of(p2 - f1.x, p3 - f1.y), c0 = transposed(l0), c1 = transposed(l1);
-                        mma_f16(O[n][i][0], u0 & 0x000f000fu, u0 & 0x00f000f0u, u1 & 0x000f000fu, u1 & 0x00f000f0u, c0, c1);
-                        mma_f16(O[n][i][1], w0 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x000f000fu, w1 & 0x00f000f0u, c0, c1);
-                        const float2 r0 = __half22float2(*(const __half2*)&l0), r1 = __half22float2(*(const __half2*)&l1);
-                        f0.x += r0.x; f0.y += r0.y; f1.x += r1.x; f1.y += r1.y;
+                        // sums of a page of their own, added in 32 bits: the tensor cores' own additions cut instead of rounding
+                        const uint32_t l0 = transposed(half2_of(p0 - f0.x, p1 - f0.y)), l1 = transposed(half2_of(p2 - f1.x, p3 - f1.y));
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            float y[4] = {0.f, 0.f, 0.f, 0.f};
+                            mma_f16(y, c[4 * h], c[4 * h + 1], c[4 * h + 2], c[4 * h + 3], l0, l1);
+                            mma_f16(y, c[4 * h], c[4 * h + 1], c[4 * h + 2], c[4 * h + 3], b0, b1);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) O[n][i][h][e] += y[e];
+                        }
+                        continue;
                     }
+                    mma_f16(O[n][i][0], c[0], c[1], c[2], c[3], b0, b1);
+                    mma_f16(O[n][i][1], c[4], c[5], c[6], c[7], b0, b1);
+                    // (the zeros are taken off with the same rounded numbers, so that a value of zero adds exactly nothing)
                     zs[n][i][0] = fmaf(f0.x, z0, fmaf(f1.x, z1, zs[n][i][0]));
                     zs[n][i][1] = fmaf(f0.y, z0, fmaf(f1.y, z1, zs[n][i][1]));
                 }
@@ -438,7 +467,7 @@ attend_kernel(const Args a) {
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
                             float2* to = (float2*)(acc + c * HD + 32 * i + 4 * g + 2 * h);
-                            float2 v = make_float2(fmaf(O[n][i][h][e], 16777216.0f, -zs[n][i][e]) * f, fmaf(O[n][i][h][2 + e], 1048576.0f, -zs[n][i][e]) * f);
+                            float2 v = make_float2(fmaf(O[n][i][h][e], PARTS == 2 ? 1.0f : 16777216.0f, -zs[n][i][e]) * f, fmaf(O[n][i][h][2 + e], PARTS == 2 ? 0.0625f : 1048576.0f, -zs[n][i][e]) * f);
                             if (f == 0.0f) v = make_float2(0.0f, 0.0f);
                             if (poison[n] >> (2 * i + e) & 1) v.x = v.y = __int_as_float(0x7fc00000);
                             if (w > 0) { v.x += to->x; v.y += to->y; }

@@ -32,71 +32,114 @@ __device__ __forceinline__ int page_of(const Place& p, int t, int pos) {
     return sp_index_ok(page, p.rg.n_pages, p.rg, 401) ? page : -1;
 }
 
+__device__ __forceinline__ void write_quad(float* to, float4 v) { *(float4*)to = v; }
+__device__ __forceinline__ void write_quad(__nv_bfloat16* to, float4 v) {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
+    *(uint2*)to = make_uint2(*(const uint32_t*)&a, *(const uint32_t*)&b);
+}
+
+constexpr int STORE_TOKENS = 4;             // of a block at most
+
 // A thread owns four neighbouring columns of a head; eight neighbouring threads a group. The angles are formed and their sine
 // and cosine taken in 64 bits, keys are rotated in 64 bits and rounded to 32 once: at position 100,000 an angle in 32 bits is
 // off by up to 0.004, and a key's code is a comparison that an error of the rotation may turn.
-template <typename TQ>
+template <typename TQ, int NG>
 __global__ void __launch_bounds__(256)
-store_kernel(const float* qkv, TQ* q_out, uint8_t* pool, Place place, const float* inv_freq, int nh, int nkv, int hd, int rd, int write_kv) {
-    __shared__ double2 turn[KV4_MAX_HD / 2];
-    const int t = blockIdx.x, pos = place.positions[t], half = rd >> 1;
-    for (int i = threadIdx.x; i < half; i += blockDim.x) {
+store_kernel(const float* qkv, TQ* q_out, uint8_t* pool, Place place, const float* inv_freq, int T, int per_block, int nh, int nkv, int rd, int write_kv) {
+    constexpr int HD = 32 * NG, PER_HEAD = HD / 4, TILE = kv4_tile_bytes(HD);
+    __shared__ double2 turns[STORE_TOKENS][HD / 2];                  // cos, sin
+    __shared__ float2 turns32[STORE_TOKENS][HD / 2];                 // the same rounded, for q
+    __shared__ int places[STORE_TOKENS][2];                          // page (or -1), place in it
+    const int t0 = blockIdx.x * per_block, n_t = min(per_block, T - t0), half = rd >> 1;
+    for (int i = threadIdx.x; i < n_t * half; i += blockDim.x) {
+        const int k = i / half, j = i - k * half;
         double s, c;
-        sincos((double)pos * (double)inv_freq[i], &s, &c);
-        turn[i] = make_double2(c, s);
+        sincos((double)place.positions[t0 + k] * (double)inv_freq[j], &s, &c);
+        turns[k][j] = make_double2(c, s);
+        turns32[k][j] = make_float2((float)c, (float)s);
+    }
+    if (threadIdx.x < n_t) {
+        const int pos = place.positions[t0 + threadIdx.x];
+        places[threadIdx.x][0] = write_kv ? page_of(place, t0 + threadIdx.x, pos) : -1;
+        places[threadIdx.x][1] = pos % KV4_PAGE;
     }
     __syncthreads();
-    const int page = write_kv ? page_of(place, t, pos) : -1;
-    const int per_head = hd >> 2, quads = (nh + (write_kv ? 2 * nkv : 0)) * per_head, groups = hd >> 5;
-    const float* x = qkv + (size_t)t * (nh + 2 * nkv) * hd;
-    // whole warps go through the loop together: eight lanes share a group (quads come in eights)
-    for (int u0 = (blockIdx.y * blockDim.x + threadIdx.x) & ~31; u0 < quads; u0 += gridDim.y * blockDim.x) {
-        const int u = u0 + (threadIdx.x & 31);
-        const bool in = u < quads;
-        const int head = in ? u / per_head : 0, d = in ? (u - head * per_head) * 4 : 0;
-        const bool is_q = head < nh, is_v = head >= nh + nkv, rotates = in && !is_v && d < rd;
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f), o = v;
-        if (in) v = *(const float4*)(x + (size_t)head * hd + d);
-        if (rotates) {
-            const bool first = d < half;
-            o = *(const float4*)(x + (size_t)head * hd + (first ? d + half : d - half));
-            const double2* tr = turn + (first ? d : d - half);
-            float* a = &v.x;
-            const float* b = &o.x;
+    const int quads = (nh + (write_kv ? 2 * nkv : 0)) * PER_HEAD;
+    for (int k = 0; k < n_t; ++k) {
+        const int page = places[k][0], slot = places[k][1];
+        const float* x = qkv + (size_t)(t0 + k) * (nh + 2 * nkv) * HD;
+        // Whole warps go through the loop together: eight lanes share a group (quads come in eights). Two quads a turn, so that the
+        // next one's columns are on their way.
+        const int stride = gridDim.y * blockDim.x;
+        for (int u0 = (blockIdx.y * blockDim.x + threadIdx.x) & ~31; u0 < quads; u0 += 2 * stride) {
+            float4 vs[2], os[2];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const double c = tr[e].x, s = first ? -tr[e].y : tr[e].y;
-                a[e] = is_q ? (float)c * a[e] + (float)s * b[e] : (float)((double)a[e] * c + (double)b[e] * s);
+            for (int i = 0; i < 2; ++i) {
+                const int u = u0 + i * stride + (threadIdx.x & 31), head = u / PER_HEAD, d = (u - head * PER_HEAD) * 4;
+                vs[i] = os[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (u < quads) {
+                    vs[i] = *(const float4*)(x + 4 * u);
+                    if (head < nh + nkv && d < rd) os[i] = *(const float4*)(x + 4 * u + (d < half ? half : -half));
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int u = u0 + i * stride + (threadIdx.x & 31);
+                const bool in = u < quads;
+                const int head = u / PER_HEAD, d = (u - head * PER_HEAD) * 4;
+                const bool is_q = head < nh, is_v = head >= nh + nkv, first = d < half;
+                float4 v = vs[i];
+                if (in && !is_v && d < rd) {
+                    const int at = first ? d : d - half;
+                    float* a = &v.x;
+                    const float* b = &os[i].x;
+                    if (is_q) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float2 w = turns32[k][at + e];
+                            a[e] = w.x * a[e] + (first ? -w.y : w.y) * b[e];
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const double2 w = turns[k][at + e];
+                            a[e] = (float)((double)a[e] * w.x + (double)b[e] * (first ? -w.y : w.y));
+                        }
+                    }
+                }
+                if (in && is_q) write_quad(q_out + ((size_t)(t0 + k) * nh + head) * HD + d, v);
+                if (!__any_sync(0xffffffffu, in && !is_q)) continue;
+                float lo = fminf(fminf(fminf(v.x, v.y), fminf(v.z, v.w)), 0.0f), hi = fmaxf(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)), 0.0f);
+                const bool bad = q4_bad(v.x) || q4_bad(v.y) || q4_bad(v.z) || q4_bad(v.w);
+#pragma unroll
+                for (int s = 1; s < 8; s *= 2) {
+                    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, s));
+                    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, s));
+                }
+                const Q4Scale g = q4_group(lo, hi, (__ballot_sync(0xffffffffu, bad) >> (threadIdx.x & 24) & 255u) != 0);
+                const int c0 = q4_code(v.x, g), c1 = q4_code(v.y, g), c2 = q4_code(v.z, g), c3 = q4_code(v.w, g);
+                const int p8 = (d >> 2) & 7, group = d >> 5;
+                // a key's word holds eight columns: two threads'
+                uint32_t word = ((uint32_t)c0 | (uint32_t)c1 << 16 | (uint32_t)c2 << 4 | (uint32_t)c3 << 20) << (8 * (p8 & 1));
+                word |= __shfl_xor_sync(0xffffffffu, word, 1);
+                if (!in || is_q || page < 0) continue;
+                uint8_t* tile = pool + ((size_t)page * nkv + (is_v ? head - nh - nkv : head - nh)) * TILE;
+                if (is_v) *(uint16_t*)(tile + kv4_v_codes(HD) + kv4_v_at(slot, p8, group, HD)) = (uint16_t)(c0 | c1 << 4 | c2 << 8 | c3 << 12);
+                else if (!(p8 & 1)) *(uint32_t*)(tile + kv4_k_at(slot, p8 >> 1, group, HD)) = word;
+                if (p8 == 0) *(uint16_t*)(tile + (is_v ? kv4_v_meta(HD) : kv4_k_meta(HD)) + ((is_v ? slot : kv4_key_slot(slot)) * NG + group) * 2) = (uint16_t)q4_meta(g);
             }
         }
-        if (in && is_q) {
-            TQ* to = q_out + ((size_t)t * nh + head) * hd + d;
-            sp_st2(to, 0, v.x, v.y);
-            sp_st2(to, 2, v.z, v.w);
-        }
-        if (!__any_sync(0xffffffffu, in && !is_q)) continue;
-        float lo = fminf(fminf(fminf(v.x, v.y), fminf(v.z, v.w)), 0.0f), hi = fmaxf(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)), 0.0f);
-        int bad = q4_bad(v.x) || q4_bad(v.y) || q4_bad(v.z) || q4_bad(v.w);
-#pragma unroll
-        for (int s = 1; s < 8; s *= 2) {
-            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, s));
-            hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, s));
-            bad |= __shfl_xor_sync(0xffffffffu, bad, s);
-        }
-        const Q4Scale g = q4_group(lo, hi, bad != 0);
-        const int c0 = q4_code(v.x, g), c1 = q4_code(v.y, g), c2 = q4_code(v.z, g), c3 = q4_code(v.w, g);
-        const int p8 = (d >> 2) & 7, group = d >> 5, slot = pos % KV4_PAGE;
-        // a key's word holds eight columns: two threads'
-        uint32_t word = ((uint32_t)c0 | (uint32_t)c1 << 16 | (uint32_t)c2 << 4 | (uint32_t)c3 << 20) << (8 * (p8 & 1));
-        word |= __shfl_xor_sync(0xffffffffu, word, 1);
-        if (!in || is_q || page < 0) continue;
-        uint8_t* tile = pool + ((size_t)page * nkv + (is_v ? head - nh - nkv : head - nh)) * kv4_tile_bytes(hd);
-        if (is_v) {
-            *(uint16_t*)(tile + kv4_v_codes(hd) + kv4_v_at(slot, p8, group, hd)) = (uint16_t)(c0 | c1 << 4 | c2 << 8 | c3 << 12);
-        } else if (!(p8 & 1)) {
-            *(uint32_t*)(tile + kv4_k_at(slot, p8 >> 1, group, hd)) = word;
-        }
-        if (p8 == 0) *(uint16_t*)(tile + (is_v ? kv4_v_meta(hd) : kv4_k_meta(hd)) + ((is_v ? slot : kv4_key_slot(slot)) * groups + group) * 2) = (uint16_t)q4_meta(g);
+    }
+}
+
+template <typename TQ>
+void launch_store(int hd, dim3 grid, cudaStream_t stream, const float* qkv, TQ* q_out, uint8_t* pool, const Place& place, const float* inv_freq, int T,
+                  int per_block, int nh, int nkv, int rd, int write_kv) {
+    switch (hd) {
+        case 32: store_kernel<TQ, 1><<<grid, 256, 0, stream>>>(qkv, q_out, pool, place, inv_freq, T, per_block, nh, nkv, rd, write_kv); break;
+        case 64: store_kernel<TQ, 2><<<grid, 256, 0, stream>>>(qkv, q_out, pool, place, inv_freq, T, per_block, nh, nkv, rd, write_kv); break;
+        case 96: store_kernel<TQ, 3><<<grid, 256, 0, stream>>>(qkv, q_out, pool, place, inv_freq, T, per_block, nh, nkv, rd, write_kv); break;
+        default: store_kernel<TQ, 4><<<grid, 256, 0, stream>>>(qkv, q_out, pool, place, inv_freq, T, per_block, nh, nkv, rd, write_kv); break;
     }
 }
 
@@ -111,12 +154,6 @@ __device__ __forceinline__ float4 read_quad(const uint8_t* tile, int slot, int d
     const uint32_t w = *(const uint32_t*)(tile + kv4_k_at(slot, p8 >> 1, group, hd)) >> (8 * (p8 & 1));
     const uint32_t m = *(const uint16_t*)(tile + kv4_k_meta(hd) + (kv4_key_slot(slot) * groups + group) * 2);
     return make_float4(q4_value(w & 15, m), q4_value((w >> 16) & 15, m), q4_value((w >> 4) & 15, m), q4_value((w >> 20) & 15, m));
-}
-
-template <typename T>
-__device__ __forceinline__ void write_quad(T* to, float4 v) {
-    sp_st2(to, 0, v.x, v.y);
-    sp_st2(to, 2, v.z, v.w);
 }
 
 template <typename T>
@@ -185,14 +222,17 @@ SP_API int sp_kv4_store(const void* qkv, void* q_out, int q_dt, void* pool, cons
     if (rd < 0 || rd > hd || rd % 8) SP_FAIL("kv4_store: rotated sizes are multiples of 8 up to the head size, got %d of %d", rd, hd);
     if (rd && !inv_freq) SP_FAIL("kv4_store: rotation needs the frequencies");
     if (write_kv && (!pool || !page_table || max_pages <= 0)) SP_FAIL("kv4_store: writing needs the pages and their table");
-    if (((uintptr_t)qkv & 15) || ((uintptr_t)q_out & 7) || ((uintptr_t)pool & 15)) SP_FAIL("kv4_store: rows and pages must start on 16-byte boundaries, q on 8");
+    if (((uintptr_t)qkv & 15) || ((uintptr_t)q_out & 15) || ((uintptr_t)pool & 15)) SP_FAIL("kv4_store: rows, q and pages must start on 16-byte boundaries");
     const Place place{token_seq, positions, seq_row, page_table, max_pages, sp_range_host};
-    const int quads = (nh + 2 * nkv) * (hd / 4), sms = sp_sm_count() > 0 ? sp_sm_count() : 148;
-    int parts = (quads + 255) / 256;                                // a few tokens: a token's heads over several blocks
-    if (T * parts > 4 * sms) parts = T >= 4 * sms ? 1 : (4 * sms + T - 1) / T;
-    const dim3 grid(T, parts);
-    if (q_dt == SP_DT_F32) store_kernel<<<grid, 256, 0, stream>>>((const float*)qkv, (float*)q_out, (uint8_t*)pool, place, inv_freq, nh, nkv, hd, rd, write_kv);
-    else store_kernel<<<grid, 256, 0, stream>>>((const float*)qkv, (__nv_bfloat16*)q_out, (uint8_t*)pool, place, inv_freq, nh, nkv, hd, rd, write_kv);
+    const int quads = (nh + (write_kv ? 2 * nkv : 0)) * (hd / 4), sms = sp_sm_count() > 0 ? sp_sm_count() : 148;
+    // a few tokens: a token's heads over several blocks; many: several tokens to a block, whose angles are formed side by side
+    int per_block = T / (16 * sms), parts = (quads + 255) / 256;
+    per_block = per_block < 1 ? 1 : per_block > STORE_TOKENS ? STORE_TOKENS : per_block;
+    const int blocks = (T + per_block - 1) / per_block;
+    if (blocks * parts > 6 * sms) parts = blocks >= 6 * sms ? 1 : (6 * sms + blocks - 1) / blocks;
+    const dim3 grid(blocks, parts < 1 ? 1 : parts);
+    if (q_dt == SP_DT_F32) launch_store(hd, grid, stream, (const float*)qkv, (float*)q_out, (uint8_t*)pool, place, inv_freq, T, per_block, nh, nkv, rd, write_kv);
+    else launch_store(hd, grid, stream, (const float*)qkv, (__nv_bfloat16*)q_out, (uint8_t*)pool, place, inv_freq, T, per_block, nh, nkv, rd, write_kv);
     SP_CHECK_LAUNCH("kv4_store");
     return 0;
 }
@@ -201,7 +241,7 @@ SP_API int sp_kv4_load(const void* pool, void* k_out, void* v_out, int dt, const
                        const int* page_table, int max_pages, int page_size, int T, int nkv, int hd, cudaStream_t stream) {
     if (T <= 0) return 0;
     if (check_heads("kv4_load", nkv, hd, page_size)) return 1;
-    if (((uintptr_t)k_out & 7) || ((uintptr_t)v_out & 7) || ((uintptr_t)pool & 15)) SP_FAIL("kv4_load: pages must start on 16-byte boundaries, rows on 8");
+    if (((uintptr_t)k_out & 15) || ((uintptr_t)v_out & 15) || ((uintptr_t)pool & 15)) SP_FAIL("kv4_load: pages and rows must start on 16-byte boundaries");
     const Place place{token_seq, positions, seq_row, page_table, max_pages, sp_range_host};
     const int parts = (2 * nkv * (hd / 4) + 255) / 256;
     const dim3 grid(T, parts);

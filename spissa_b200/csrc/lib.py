@@ -47,6 +47,10 @@ def load(module: str) -> ctypes.CDLL:
             # declared once: plain integers pass, without an object made for each of a call's arguments
             lib.sp_q4_gemv.argtypes = [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_longlong,
                                        c_longlong, c_int, c_int, c_float, c_void_p]
+        if module == "kv4":
+            lib.sp_kv4_store.argtypes = [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p] + \
+                [c_int] * 6 + [c_void_p]
+            lib.sp_kv4_load.argtypes = [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p] + [c_int] * 5 + [c_void_p]
         if module == "kv4_attention":
             lib.sp_kv4_attend.argtypes = [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p] + [c_int] * 9 + \
                 [c_float, c_void_p, c_int, c_int, c_int, c_void_p, c_longlong, c_void_p, c_void_p]
@@ -1777,7 +1781,7 @@ def _on_one_device(what: str, *ts) -> None:
     """A launch goes to the current device's stream: its tensors have to live there."""
     here = torch.cuda.current_device()
     for t in ts:
-        if t is not None and (not t.is_cuda or t.device.index != here):
+        if t is not None and t.get_device() != here:
             raise KernelError(f"{what}: tensors on the current device (cuda:{here}) are wanted, got one on {t.device}")
 
 
@@ -1857,16 +1861,26 @@ def kv4_pool(n_pages: int, nkv: int, hd: int, device) -> torch.Tensor:
     return torch.zeros(int(n_pages), int(nkv), kv4_tile_bytes(hd), dtype=torch.uint8, device=device)
 
 
+_I32 = torch.int32
+
+
 def _kv4_check(what: str, pool, meta, T: int, nkv: int, hd: int, *ts) -> None:
-    if pool.dtype != torch.uint8 or pool.dim() != 3 or pool.shape[1] != nkv or pool.shape[2] != kv4_tile_bytes(hd):
+    seqs, positions, rows, table = meta.token_seq, meta.positions, meta.seq_slot, meta.page_table
+    if pool.dtype != torch.uint8 or pool.dim() != 3 or pool.size(1) != nkv or pool.size(2) != kv4_tile_bytes(hd):
         raise KernelError(f"{what}: pages are uint8 [pages, {nkv}, {kv4_tile_bytes(hd)}], got {pool.dtype} {tuple(pool.shape)}")
     if meta.page_size != 64:
         raise KernelError(f"{what}: pages of 64 positions, got {meta.page_size}")
-    tables = (meta.token_seq, meta.positions, meta.seq_slot, meta.page_table)
-    if any(t.dtype != torch.int32 for t in tables) or meta.page_table.dim() != 2 or min(meta.token_seq.numel(), meta.positions.numel()) < T:
+    if not (seqs.dtype == positions.dtype == rows.dtype == table.dtype == _I32) or table.dim() != 2 or seqs.size(0) < T or positions.size(0) < T:
         raise KernelError(f"{what}: the step's arrays are int32, one sequence and position a token, pages [sequences, entries]")
-    _need_contig(pool, *tables, *ts)
-    _on_one_device(what, pool, *tables, *ts)
+    here = pool.get_device()
+    if not (here == seqs.get_device() == positions.get_device() == rows.get_device() == table.get_device()) or here < 0 \
+            or here != torch._C._cuda_getDevice():
+        raise KernelError(f"{what}: the pages and the step's arrays live on the current device, got {pool.device}, {positions.device}, {table.device}")
+    if not (pool.is_contiguous() and seqs.is_contiguous() and positions.is_contiguous() and rows.is_contiguous() and table.is_contiguous()):
+        raise KernelError("kernels take contiguous tensors")
+    for t in ts:
+        if t is not None and (t.get_device() != here or not t.is_contiguous()):
+            raise KernelError(f"{what}: contiguous tensors on the current device are wanted, got one on {t.device}")
 
 
 def kv4_store(qkv, q_out, pool, meta, inv_freq, nh, nkv, hd, rd, write_kv=True) -> None:
@@ -1876,33 +1890,38 @@ def kv4_store(qkv, q_out, pool, meta, inv_freq, nh, nkv, hd, rd, write_kv=True) 
     T = qkv.shape[0]
     if qkv.dtype != torch.float32 or qkv.dim() != 2 or qkv.shape[1] != (nh + 2 * nkv) * hd:
         raise KernelError(f"kv4_store: rows of {nh} + 2 x {nkv} heads of {hd} in float32 are wanted, got {qkv.dtype} {tuple(qkv.shape)}")
-    if (q_out is None) != (nh == 0) or (q_out is not None and tuple(q_out.shape) != (T, nh * hd)):
+    if (q_out is None) != (nh == 0) or (nh and q_out.shape != (T, nh * hd)):
         raise KernelError(f"kv4_store: q goes to a tensor [{T}, {nh * hd}]")
     if rd and (inv_freq is None or inv_freq.dtype != torch.float32 or inv_freq.numel() < rd // 2):
         raise KernelError(f"kv4_store: rotating {rd} dims takes {rd // 2} float32 frequencies")
     _kv4_check("kv4_store", pool, meta, T, nkv, hd, qkv, q_out, inv_freq)
     lib = load("kv4")
     pt = meta.page_table
-    _declare_bounds("kv4", lib, _pool_pages(meta, pool), _table_rows(meta, pt), qkv.device)
-    _check("kv4", lib.sp_kv4_store(
-        c_void_p(_ptr(qkv)), c_void_p(_ptr(q_out)), dt_code(q_out) if q_out is not None else F32, c_void_p(_ptr(pool)),
-        c_void_p(_ptr(meta.token_seq)), c_void_p(_ptr(meta.positions)), c_void_p(_ptr(meta.seq_slot)), c_void_p(_ptr(pt)), pt.shape[1],
-        meta.page_size, c_void_p(_ptr(inv_freq)), T, int(nh), int(nkv), int(hd), int(rd), int(bool(write_kv)), c_void_p(_stream())))
+    if _RANGE_CHECKED["kv4"]:
+        _declare_bounds("kv4", lib, _pool_pages(meta, pool), _table_rows(meta, pt), qkv.device)
+    rc = lib.sp_kv4_store(
+        qkv.data_ptr(), q_out.data_ptr() if nh else None, dt_code(q_out) if nh else F32, pool.data_ptr(), meta.token_seq.data_ptr(),
+        meta.positions.data_ptr(), meta.seq_slot.data_ptr(), pt.data_ptr(), pt.shape[1], meta.page_size,
+        inv_freq.data_ptr() if rd else None, T, nh, nkv, hd, rd, bool(write_kv), _stream())
+    if rc:
+        _check("kv4", rc)
 
 
 def kv4_load(pool, meta, k_out, v_out, nkv, hd) -> None:
     """k_out, v_out [T, nkv, hd] (float32 or bfloat16, which holds them exactly) = what the pages hold of the step's tokens."""
     T = k_out.shape[0]
-    if tuple(k_out.shape) != (T, nkv, hd) or v_out.shape != k_out.shape or v_out.dtype != k_out.dtype:
+    if k_out.shape != (T, nkv, hd) or v_out.shape != k_out.shape or v_out.dtype != k_out.dtype:
         raise KernelError(f"kv4_load: keys and values go to two tensors [tokens, {nkv}, {hd}] of one type")
     _kv4_check("kv4_load", pool, meta, T, nkv, hd, k_out, v_out)
     lib = load("kv4")
     pt = meta.page_table
-    _declare_bounds("kv4", lib, _pool_pages(meta, pool), _table_rows(meta, pt), pool.device)
-    _check("kv4", lib.sp_kv4_load(
-        c_void_p(_ptr(pool)), c_void_p(_ptr(k_out)), c_void_p(_ptr(v_out)), dt_code(k_out), c_void_p(_ptr(meta.token_seq)),
-        c_void_p(_ptr(meta.positions)), c_void_p(_ptr(meta.seq_slot)), c_void_p(_ptr(pt)), pt.shape[1], meta.page_size, T, int(nkv),
-        int(hd), c_void_p(_stream())))
+    if _RANGE_CHECKED["kv4"]:
+        _declare_bounds("kv4", lib, _pool_pages(meta, pool), _table_rows(meta, pt), pool.device)
+    rc = lib.sp_kv4_load(
+        pool.data_ptr(), k_out.data_ptr(), v_out.data_ptr(), dt_code(k_out), meta.token_seq.data_ptr(), meta.positions.data_ptr(),
+        meta.seq_slot.data_ptr(), pt.data_ptr(), pt.shape[1], meta.page_size, T, nkv, hd, _stream())
+    if rc:
+        _check("kv4", rc)
 
 
 def kv4_unpack_pages(pool, meta, k_out, v_out, table, step, window, nkv, hd) -> None:
@@ -1938,7 +1957,7 @@ def kv4_attend(q, pool, out, meta, seq_start, n_seqs: int, max_new: int, longest
     ``seq_start`` [n_seqs + 1] int32, or None where every sequence brings one token; ``max_new``: the most tokens of a sequence;
     ``longest``: the keys that the longest sequence may have (it shapes the split of the keys)."""
     T = q.shape[0]
-    if q.dtype not in _DT or tuple(q.shape) != (T, nh * hd) or out.shape != q.shape or out.dtype != q.dtype or nh % nkv:
+    if q.dtype not in _DT or q.shape != (T, nh * hd) or out.shape != q.shape or out.dtype != q.dtype or nh % nkv:
         raise KernelError(f"kv4_attend: queries and output are [tokens, {nh} x {hd}] of one type, of heads in equal groups")
     if sink is not None and (sink.dtype != torch.float32 or sink.numel() != nh):
         raise KernelError("kv4_attend: the sinks are one float32 per query head")
@@ -1954,7 +1973,8 @@ def kv4_attend(q, pool, out, meta, seq_start, n_seqs: int, max_new: int, longest
     nt, chunk_pages, n_chunks = plan or kv4_attend_plan(n_seqs, nkv, max_new * (nh // nkv), max(1, pages))
     need = T * nh * n_chunks * (hd + 2) if n_chunks > 1 else 0
     scratch = torch.empty(need, dtype=torch.float32, device=q.device) if need else None
-    _declare_bounds("kv4_attention", lib, _pool_pages(meta, pool), _table_rows(meta, pt), q.device)
+    if _RANGE_CHECKED["kv4_attention"]:
+        _declare_bounds("kv4_attention", lib, _pool_pages(meta, pool), _table_rows(meta, pt), q.device)
     rc = lib.sp_kv4_attend(
         q.data_ptr(), out.data_ptr(), dt_code(q), pool.data_ptr(), seq_start.data_ptr() if seq_start is not None else None,
         meta.positions.data_ptr(), meta.seq_slot.data_ptr(), pt.data_ptr(), pt.shape[1], meta.page_size, T, n_seqs, max_new, nh, nkv, hd, window,

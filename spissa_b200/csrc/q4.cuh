@@ -16,12 +16,20 @@
 // front a code is the bfloat16 128 + c, and 128 + c minus 128 + z is exact.
 #pragma once
 #include "common.cuh"
+#include <cuda_fp16.h>
 
 namespace {
 
 __device__ __forceinline__ uint32_t q4_pair(uint32_t word, int j) { return ((word >> (4 * j)) & 0x000f000fu) | 0x43004300u; }
 __device__ __forceinline__ float q4_scale_of(uint32_t meta) { return __uint_as_float((meta & 0xfff0u) << 16); }
 __device__ __forceinline__ float q4_value(int code, uint32_t meta) { return q4_scale_of(meta) * (float)(code - (int)(meta & 15u)); }
+
+// c − z as two float16 numbers, exactly, from the bits (w & 0x000f000f, or w & 0x00f000f0: 16 c) and z (16 z) in the same places
+__device__ __forceinline__ uint32_t q4_less(uint32_t c, uint32_t z) {
+    const uint32_t a = c | 0x64006400u, b = z | 0x64006400u;         // 1024 + c, 1024 + z
+    const __half2 r = __hsub2(*(const __half2*)&a, *(const __half2*)&b);
+    return *(const uint32_t*)&r;
+}
 
 __device__ __forceinline__ uint32_t bf2_sub(uint32_t a, uint32_t b) {
     const __nv_bfloat162 r = __hsub2(*(const __nv_bfloat162*)&a, *(const __nv_bfloat162*)&b);
@@ -34,31 +42,42 @@ __device__ __forceinline__ uint32_t bf2_mul(uint32_t a, uint32_t b) {
 
 struct Q4Scale { float s, inv; int z; };
 
-// s and z of a group from its bounds (lo <= 0 <= hi), in 64 bits: hi − lo and the quotients are compared with values that
-// they may equal (a multiple of s halfway between two codes, a power of two's boundary).
+// round(x / s), ties to even, |x / s| < 2^20: a quotient by the reciprocal, rounded in the place of ones of 1.5 · 2^23 and at most
+// one off; the remainder x − s·t, which is exact (s·t has eight bits and x's last place is below s's), decides.
+__device__ __forceinline__ int q4_round(float x, float s, float inv) {
+    const float y = fmaf(x, inv, 12582912.0f), d = fmaf(-s, y - 12582912.0f, x), over = 2.0f * fabsf(d) - s;
+    int t = __float_as_int(y) - 0x4b400000;
+    if (over >= 0.0f && (over > 0.0f || (t & 1))) t += d > 0.0f ? 1 : -1;      // (over is exact: both are multiples of x's last place)
+    return t;
+}
+
+// (hi − lo) / 15 rounded up to four significant bits, or 0 below 2^-100, in 64 bits: a range may be a multiple of 15 exactly
+static __device__ __noinline__ float q4_step(float lo, float hi) {
+    const double r = (double)hi - (double)lo;
+    if (r < 7.888609052210118e-31) return 0.0f;
+    constexpr long long LOW = (1ll << 49) - 1;                       // all but four significant bits
+    return (float)__longlong_as_double((__double_as_longlong(r / 15.0) + LOW) & ~LOW);
+}
+
+// s and z of a group from its bounds (lo <= 0 <= hi). The quotient in 32 bits is off by at most four of its last places, so
+// rounding it up gives the same unless it lies within 16 of a number of four bits.
 __device__ __forceinline__ Q4Scale q4_group(float lo, float hi, bool bad) {
     Q4Scale g{0.0f, 0.0f, 0};
-    const double r = (double)hi - (double)lo;
     if (bad) { g.s = __int_as_float(0x7fc00000); return g; }
-    if (r < 7.888609052210118e-31) return g;                         // 2^-100
-    long long bits = __double_as_longlong(r / 15.0);
-    constexpr long long LOW = (1ll << 49) - 1;                       // all but four significant bits
-    bits = (bits + LOW) & ~LOW;
-    const double s = __longlong_as_double(bits);
-    g.s = (float)s;
-    g.inv = 1.0f / g.s;
-    g.z = __double2int_rn(-(double)lo / s);
+    const float r = hi - lo;
+    const uint32_t q = __float_as_uint(r * (1.0f / 15.0f)), low = q & 0xfffffu;
+    g.s = __uint_as_float((q & ~0xfffffu) + 0x100000u);
+    if (low - 16u > 0xfffffu - 32u || r < 1.6e-30f) g.s = q4_step(lo, hi);
+    if (g.s > 0.0f) {
+        asm("rcp.approx.f32 %0, %1;" : "=f"(g.inv) : "f"(g.s));
+        g.z = q4_round(-lo, g.s, g.inv);
+    }
     return g;
 }
 
-// The code of x: a quotient by the reciprocal, at most one off, and the remainder x − s·t, which is exact (s·t has eight
-// bits and x's last place is below s's), decides.
 __device__ __forceinline__ int q4_code(float x, const Q4Scale& g) {
     if (!(g.s > 0.0f)) return 0;                                     // zeros, NaN
-    float t = rintf(x * g.inv);
-    const float d = fmaf(-g.s, t, x), over = 2.0f * fabsf(d) - g.s;  // exact: both are multiples of x's last place
-    if (over > 0.0f || (over == 0.0f && ((int)t & 1))) t += copysignf(1.0f, d);
-    return min(15, max(0, (int)t + g.z));
+    return min(15, max(0, q4_round(x, g.s, g.inv) + g.z));
 }
 
 __device__ __forceinline__ uint32_t q4_meta(const Q4Scale& g) { return ((__float_as_uint(g.s) >> 16) & 0xfff0u) | (uint32_t)g.z; }

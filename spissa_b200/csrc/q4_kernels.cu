@@ -84,7 +84,8 @@ __global__ void unpack_kernel(const uint32_t* codes, const uint16_t* meta, T* ou
 // half of that, but m16n8k32 on those runs at half the rate of two on float16 here.)
 // x is multiplied by a power of two per row and block of 128 columns that brings the block's largest entry into 2^14 .. 2^15:
 // exact for bfloat16 entries down to 2^-26 of the block's largest, off by 2^-39 of the largest below. float32 entries are two
-// float16 numbers each, 22 bits. (Blocks whose largest entry lies outside 2^-80 .. 2^100 overflow or vanish.) The zero is taken off
+// float16 numbers each, 22 bits, and meet c − z itself, as 1024 + c less 1024 + z: tensor cores cut partial sums to 24 bits
+// instead of rounding them, and sums of x c are many times those of x (c − z). (Blocks whose largest entry lies outside 2^-80 .. 2^100 overflow or vanish.) The zero is taken off
 // the sums, Σ x (c − z) = Σ x c − z Σ x, with Σ x per group in 32 bits, and a group's sum is scaled in 32 bits. A row with
 // an entry that is not finite gives NaN.
 //
@@ -211,7 +212,7 @@ gemv_kernel(const TX* x, const Product p) {
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
             const int up = top > 0.0f ? min(94, max(-94, 141 - (int)(__float_as_uint(top) >> 23))) : 0;
-            const float scale = __uint_as_float((uint32_t)(127 + up) << 23), unit = __uint_as_float((uint32_t)(151 - up) << 23);
+            const float scale = __uint_as_float((uint32_t)(127 + up) << 23), unit = __uint_as_float((uint32_t)((PARTS == 2 ? 127 : 151) - up) << 23);
             by[n] = make_float2(__shfl_sync(0xffffffffu, unit, 8 * t), __shfl_sync(0xffffffffu, unit, 8 * t + 4));
             float sum = 0.0f;
 #pragma unroll
@@ -264,12 +265,20 @@ gemv_kernel(const TX* x, const Product p) {
                             for (int r = 0; r < RT; ++r) {
                                 const uint4 c = w[d][r][q >> 1];
                                 const uint32_t r0 = (q & 1 ? c.y : c.x) >> (8 * half), r1 = (q & 1 ? c.w : c.z) >> (8 * half);
+                                uint32_t a0 = r0 & 0x000f000fu, a1 = r1 & 0x000f000fu, a2 = r0 & 0x00f000f0u, a3 = r1 & 0x00f000f0u;
+                                if (PARTS == 2) {
+                                    const uint32_t mm = m[d][r][q / (GROUP / 32)], z0 = (mm & 15u) * 0x10001u, z1 = ((mm >> 16) & 15u) * 0x10001u;
+                                    a0 = q4_less(a0, z0);
+                                    a1 = q4_less(a1, z1);
+                                    a2 = q4_less(a2, z0 << 4);
+                                    a3 = q4_less(a3, z1 << 4);
+                                }
 #pragma unroll
                                 for (int n = 0; n < NT; ++n)
 #pragma unroll
                                     for (int part = PARTS - 1; part >= 0; --part) {
                                         const uint4 v = xv[n][q][part];
-                                        mma_f16(acc[r][n], r0 & 0x000f000fu, r1 & 0x000f000fu, r0 & 0x00f000f0u, r1 & 0x00f000f0u, half ? v.z : v.x, half ? v.w : v.y);
+                                        mma_f16(acc[r][n], a0, a1, a2, a3, half ? v.z : v.x, half ? v.w : v.y);
                                     }
                             }
                         if ((q + 1) % (GROUP / 32) == 0) {
@@ -278,9 +287,16 @@ gemv_kernel(const TX* x, const Product p) {
                             for (int r = 0; r < RT; ++r) {
                                 const uint32_t mm = m[d][r][i];
                                 const float s0 = __uint_as_float((mm << 16) & 0xfff00000u), s1 = __uint_as_float(mm & 0xfff00000u);
-                                const float z0 = (float)(mm & 15u), z1 = (float)((mm >> 16) & 15u);
+                                const float z0 = PARTS == 2 ? 0.0f : (float)(mm & 15u), z1 = PARTS == 2 ? 0.0f : (float)((mm >> 16) & 15u);
 #pragma unroll
                                 for (int n = 0; n < NT; ++n) {
+                                    if (PARTS == 2) {
+                                        y[r][n].x = fmaf(s0, acc[r][n][0], y[r][n].x);
+                                        y[r][n].y = fmaf(s0, acc[r][n][1], y[r][n].y);
+                                        y[r][n].z = fmaf(s1, acc[r][n][2], y[r][n].z);
+                                        y[r][n].w = fmaf(s1, acc[r][n][3], y[r][n].w);
+                                        continue;
+                                    }
                                     y[r][n].x = fmaf(s0, fmaf(z0, sx[n][i].x, acc[r][n][0]), y[r][n].x);
                                     y[r][n].y = fmaf(s0, fmaf(z0, sx[n][i].y, acc[r][n][1]), y[r][n].y);
                                     y[r][n].z = fmaf(s1, fmaf(z1, sx[n][i].x, acc[r][n][2]), y[r][n].z);

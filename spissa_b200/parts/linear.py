@@ -175,9 +175,8 @@ class Linear4:
         if out is None:
             if accumulate:
                 raise ValueError("accumulation needs the tensor to add into")
-            out = torch.empty(x.shape[0], self.out_features, dtype=out_dtype or x.dtype, device=x.device)
-        check4(self, x, out, self.out_features, accumulate)
-        M = x.shape[0]
+            out = x.new_empty((x.shape[0], self.out_features), dtype=out_dtype)
+        M = check4(self, x, out, self.out_features, accumulate)
         if 0 < M <= K.Q4_GEMV_ROWS:
             K.q4_gemv(on_boundaries(x), self.codes, self.scales, out, self.out_features, self.group, 0, K.TC_ACCUMULATE if accumulate else K.TC_STORE)
         elif M:
@@ -209,9 +208,8 @@ class GatedLinear4:
         return plain
 
     def __call__(self, x: torch.Tensor, act_dtype) -> torch.Tensor:
-        out = torch.empty(x.shape[0], self.intermediate, dtype=act_dtype, device=x.device)
-        check4(self, x, out, self.intermediate, False)
-        M = x.shape[0]
+        out = x.new_empty((x.shape[0], self.intermediate), dtype=act_dtype)
+        M = check4(self, x, out, self.intermediate, False)
         if 0 < M <= K.Q4_GEMV_ROWS:
             K.q4_gemv(on_boundaries(x), self.codes, self.scales, out, 2 * self.intermediate, self.group, self.intermediate, K.TC_SILU_MUL, self.act, self.mult)
         elif M:
@@ -219,22 +217,23 @@ class GatedLinear4:
         return out
 
 
-def check4(lin, x, out, out_features: int, accumulate: bool) -> None:
-    """Refuses what the products of four-bit weights do not take."""
+_ROWS = (torch.bfloat16, torch.float32)
+
+
+def check4(lin, x, out, out_features: int, accumulate: bool) -> int:
+    """Refuses what the products of four-bit weights do not take; the number of rows."""
     if x.dtype not in _ROWS or out.dtype not in _ROWS or (accumulate and out.dtype != torch.float32):
         raise K.KernelError(f"products of four-bit weights take bfloat16 or float32 rows, are stored as either and added into float32; got "
                             f"{x.dtype} rows and a {out.dtype} output")
-    if x.dim() != 2 or x.shape[1] != lin.in_features or tuple(out.shape) != (x.shape[0], out_features):
+    if x.dim() != 2 or x.shape[1] != lin.in_features or out.shape != (x.shape[0], out_features):
         raise K.KernelError(f"shapes do not match: x {tuple(x.shape)}, weight [{out_features}, {lin.in_features}], out {tuple(out.shape)}")
     if x.stride(1) != 1 or out.stride(1) != 1:
         raise K.KernelError("product operands must have unit stride in their last dimension")
-    if not (x.device == out.device == lin.codes.device and x.device.index == torch.cuda.current_device()):
+    if not (x.get_device() == out.get_device() == lin.codes.get_device() == torch._C._cuda_getDevice()):
         raise K.KernelError(f"the weight (on {lin.codes.device}), its rows and its output live on the current device, got {x.device} and {out.device}")
-
-
-_ROWS = (torch.bfloat16, torch.float32)
+    return x.shape[0]
 
 
 def on_boundaries(x):
     """``x``, or a copy of it where its rows do not start on 16-byte boundaries (columns of wider rows, an odd offset)."""
-    return x if x.data_ptr() % 16 == 0 and (x.stride(0) * x.element_size()) % 16 == 0 else x.clone(memory_format=torch.contiguous_format)
+    return x if (x.data_ptr() | x.stride(0) * x.element_size()) % 16 == 0 else x.clone(memory_format=torch.contiguous_format)
