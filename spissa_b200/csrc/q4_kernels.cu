@@ -63,17 +63,41 @@ __global__ void pack_kernel(const void* w, int dt, long long ldw, uint32_t* code
     if ((8 * k8) % group == 0) meta[meta_at(row, k8, blocks, group)] = (uint16_t)q4_meta(g);
 }
 
-template <typename T>
-__global__ void unpack_kernel(const uint32_t* codes, const uint16_t* meta, T* out, int rows, int K, int blocks, int group, RowMap map) {
-    const int row = blockIdx.x, k8 = blockIdx.y * blockDim.x + threadIdx.x;
-    const int dst = source_row(row, rows, map);
-    if (dst < 0 || 8 * k8 >= K) return;
-    const uint32_t word = codes[word_at(row, k8, blocks)];
-    const uint32_t m = meta[meta_at(row, k8, blocks, group)];
-    T* to = out + (size_t)dst * K + 8 * k8;
+// The numbers themselves, a warp a block of a tile at a time: its codes in two loads, eight neighbouring numbers in one store.
+// c − z and its product with s are exact in bfloat16.
+__device__ __forceinline__ void store_eight(__nv_bfloat16* to, const uint32_t (&v)[4]) { *(uint4*)to = make_uint4(v[0], v[1], v[2], v[3]); }
+__device__ __forceinline__ void store_eight(float* to, const uint32_t (&v)[4]) {
 #pragma unroll
-    for (int i = 0; i < 8; i += 2)
-        sp_st2(to, i, q4_value((word >> (2 * i)) & 15, m), q4_value((word >> (2 * i + 16)) & 15, m));
+    for (int h = 0; h < 2; ++h)
+        *(float4*)(to + 4 * h) = make_float4(__uint_as_float(v[2 * h] << 16), __uint_as_float(v[2 * h] & 0xffff0000u),
+                                             __uint_as_float(v[2 * h + 1] << 16), __uint_as_float(v[2 * h + 1] & 0xffff0000u));
+}
+template <typename T>
+__global__ void __launch_bounds__(256)
+unpack_kernel(const uint4* codes, const uint16_t* meta, T* out, int rows, int K, int blocks, int group, RowMap map) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, tile = blockIdx.x, block = blockIdx.y * 8 + (threadIdx.x >> 5);
+    if (block >= blocks) return;
+    const uint4* from = codes + ((size_t)tile * blocks + block) * 64 + lane;
+    const uint4 w[2] = {from[0], from[32]};
+    const int per = BLOCK / group;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        const int dst = source_row(tile * 16 + g + 8 * r, rows, map);
+        if (dst < 0) continue;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {                                // quarters of 32 columns
+            const int k = block * BLOCK + 32 * i + 8 * t;
+            if (k >= K) break;
+            const uint32_t m = meta[((((size_t)tile * blocks + block) * 8 + g) * per + 32 * i / group) * 2 + r];
+            const uint32_t z = 0x43004300u | (m & 15u) * 0x10001u, s = (m & 0xfff0u) * 0x10001u;
+            const uint4 c = w[i >> 1];
+            const uint32_t word = r ? (i & 1 ? c.w : c.z) : (i & 1 ? c.y : c.x);
+            uint32_t v[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = bf2_mul(bf2_sub(q4_pair(word, j), z), s);
+            store_eight(out + (size_t)dst * K + k, v);
+        }
+    }
 }
 
 // ---------------------------------------------------------------- the product for a few tokens
@@ -433,9 +457,10 @@ SP_API int sp_q4_unpack(const void* codes, const void* meta, void* out, int dt, 
     if (check_sizes("q4_unpack", rows, K, group, half, block)) return 1;
     if ((uintptr_t)out & 15) SP_FAIL("q4_unpack: the output must start on a 16-byte boundary");
     const int packed = sp_q4_packed_rows(rows, half), blocks = (K + BLOCK - 1) / BLOCK;
-    const dim3 grid(packed, (blocks * 16 + 127) / 128);
-    if (dt == SP_DT_F32) unpack_kernel<<<grid, 128, 0, stream>>>((const uint32_t*)codes, (const uint16_t*)meta, (float*)out, rows, K, blocks, group, RowMap{half, block});
-    else unpack_kernel<<<grid, 128, 0, stream>>>((const uint32_t*)codes, (const uint16_t*)meta, (__nv_bfloat16*)out, rows, K, blocks, group, RowMap{half, block});
+    const dim3 grid(packed / 16, (blocks + 7) / 8), block_dim(blocks < 8 ? blocks * 32 : 256);
+    const RowMap map{half, block};
+    if (dt == SP_DT_F32) unpack_kernel<<<grid, block_dim, 0, stream>>>((const uint4*)codes, (const uint16_t*)meta, (float*)out, rows, K, blocks, group, map);
+    else unpack_kernel<<<grid, block_dim, 0, stream>>>((const uint4*)codes, (const uint16_t*)meta, (__nv_bfloat16*)out, rows, K, blocks, group, map);
     SP_CHECK_LAUNCH("q4_unpack");
     return 0;
 }
