@@ -8,6 +8,7 @@ same needs form a *group* with storage of its own:
   a page allocator. A sequence holds ceil(len / page_size) pages of the group, taken
   when it grows and returned when its slot is released. A windowed group returns
   pages that have fallen wholly out of the window after each step.
+  Asked for in four bits it owns one pool of bytes, ``k``, [caches, pages, kv heads, bytes of a page].
 * a state group owns ``state`` [caches, slots, *shape]; a slot's rows are zeroed when
   the slot is acquired.
 
@@ -32,6 +33,7 @@ from dataclasses import dataclass, field
 
 import torch
 
+from ..csrc.lib import kv4_tile_bytes
 from ..parts.base import CacheBundle, KVCacheRequest, StateRequest
 from .slots import CacheFull, CacheMisuse, IndexPool
 from .views import BundleView, KVLayerView, StateLayerView
@@ -79,10 +81,16 @@ class KVGroup:
         self.pages = IndexPool(n_pages, f"page of cache group {name}")
         shape = (len(self.cache_ids), n_pages, request.num_kv_heads, page_size, request.head_dim)
         v_shape = shape[:-1] + (request.v_head_dim or request.head_dim,)
+        if request.bits == 4:
+            if page_size != 64 or request.keys_only or request.v_head_dim not in (None, request.head_dim):
+                raise ValueError("four-bit pages hold 64 keys and values of one size")
+            shape, dtype = shape[:3] + (kv4_tile_bytes(request.head_dim),), torch.uint8
+        elif request.bits != 16:
+            raise ValueError(f"keys and values are cached in the activations' type (16) or in 4 bits, not in {request.bits}")
         # zeros: a masked key's weight of zero must never meet a NaN left in fresh memory
         self.k = torch.zeros(shape, dtype=dtype, device=device) if allocate else None
-        if request.keys_only:
-            self.v = self.k                              # one row per position, read as key and as value
+        if request.keys_only or request.bits == 4:
+            self.v = self.k                              # one row per position, read as key and as value; or pages of both
         else:
             self.v = torch.zeros(v_shape, dtype=dtype, device=device) if allocate else None
         self.index = {c: i for i, c in enumerate(self.cache_ids)}
@@ -93,7 +101,7 @@ class KVGroup:
     def bytes(self) -> int:
         if self.k is None:
             return 0
-        return (self.k.numel() + (0 if self.request.keys_only else self.v.numel())) * self.k.element_size()
+        return (self.k.numel() + (0 if self.v is self.k else self.v.numel())) * self.k.element_size()
 
 
 class StateGroup:
@@ -351,7 +359,7 @@ class CacheManager:
             g = self.kv_groups[gname]
             i = g.index[cache_id]
             return KVLayerView(g.k[i], g.v[i], step.page_tables[gname], self.page_size, step.token_seq,
-                               step.positions, step.seq_row, g.request.window, writes)
+                               step.positions, step.seq_row, g.request.window, writes, g.request.bits)
         g = self.state_groups[gname]
         return StateLayerView(g.state[g.index[cache_id]], writes)
 

@@ -7,7 +7,7 @@
 Option names and meanings follow ``spissa chat`` (crates/spissa-cli/src/main.rs:271-327):
 ``--ctx`` cache cap in tokens (default 2048), ``--max-new-tokens`` (chat 512), ``--temp`` (0 =
 greedy), ``--top-p`` (0.95, used when --temp > 0), ``--top-k`` (0 = no cap), ``--seed`` (0),
-``--chat-template`` (llama3 | raw), ``--system``; ``--token-ids`` and ``--logits-out`` as in
+``--weight-bits`` and ``--cache-bits`` (16 | 4, not in the reference); ``--chat-template`` (llama3 | raw), ``--system``; ``--token-ids`` and ``--logits-out`` as in
 ``spissa run`` (main.rs:133-195). ``--repeat-penalty`` exists in the reference for its Qwen
 chat only and is not offered here.
 """
@@ -27,6 +27,10 @@ def _sampling_args(p, max_new_default):
     p.add_argument("--top-k", type=int, default=0, dest="top_k", help="keep the K most probable tokens (0 = no cap)")
     p.add_argument("--seed", type=int, default=0, help="seed of the sampling draws")
     p.add_argument("--dtype", default="bf16", choices=["bf16", "fp32", "bfloat16", "float32"])
+    p.add_argument("--weight-bits", type=int, default=16, choices=[16, 4], dest="weight_bits",
+                   help="4: hold the layers' matrices in four bits a number (16: as they come)")
+    p.add_argument("--cache-bits", type=int, default=16, choices=[16, 4], dest="cache_bits",
+                   help="4: hold keys and values in four bits a number")
     p.add_argument("--device", default="cuda:0")
     p.add_argument("--profile-phases", action="store_true", dest="profile_phases",
                    help="time every phase of the block with CUDA events (steps then run kernel by kernel, part by part) "
@@ -41,11 +45,11 @@ def _engine(args, n_seqs):
         folder = tempfile.mkdtemp(prefix="spissa_b200_random_")
         write_random_model(cfg, folder, seed=args.weights_seed)
         return Engine.from_folder(folder, dtype=args.dtype, max_tokens=max_tokens, max_seqs=max(1, n_seqs),
-                                  device=args.device)
+                                  device=args.device, weight_bits=args.weight_bits, cache_bits=args.cache_bits)
     if not args.model:
         raise SystemExit("give a model folder or --random CONFIG.json")
     return Engine.from_folder(args.model, dtype=args.dtype, max_tokens=max_tokens, max_seqs=max(1, n_seqs),
-                              device=args.device)
+                              device=args.device, weight_bits=args.weight_bits, cache_bits=args.cache_bits)
 
 
 def _phase_report(engine) -> dict:

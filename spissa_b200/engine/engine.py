@@ -83,13 +83,18 @@ class Engine:
     greedy_steps = True            # ``step`` and ``step_device`` take ``greedy=True`` and return tokens instead of logits
 
     def __init__(self, config, tensors: dict, dtype, max_tokens: int, max_seqs: int | None = None,
-                 device="cuda:0", use_graphs: bool = True, fuse_decode: bool = True, fuse_prefill: bool = True):
+                 device="cuda:0", use_graphs: bool = True, fuse_decode: bool = True, fuse_prefill: bool = True,
+                 weight_bits: int = 16, cache_bits: int = 16):
+        """``weight_bits`` / ``cache_bits`` of 4 (16: as they come): the layers' matrices, and keys and values, are held in
+        four bits a number with a scale and a zero for every 64 (32) of them; embedding, norms and head stay as they are.
+        Steps then run part by part; models whose layers have parts without such a form are refused."""
         self.device = _require_gpu(device)
         self.config = config
         self.dtype = _DTYPES[dtype]
-        self.rt = Runtime(self.device, self.dtype, self.PAGE_SIZE)
+        self.rt = Runtime(self.device, self.dtype, self.PAGE_SIZE, int(weight_bits), int(cache_bits))
         self.model = Model(config.to_spec())
-        kernel_build.prefetch(self.model.kernel_modules(self.dtype))      # in the background, while the weights go up
+        self.model.check_bits(self.rt.weight_bits, self.rt.cache_bits)
+        kernel_build.prefetch(self.model.kernel_modules(self.dtype, self.rt))      # in the background, while the weights go up
         self.model.fuse_decode = fuse_decode
         self.model.fuse_prefill = fuse_prefill
         with torch.cuda.device(self.device):
@@ -122,26 +127,27 @@ class Engine:
     @classmethod
     def from_folder(cls, folder, dtype="bfloat16", max_tokens: int = 4096, max_seqs: int | None = None,
                     device="cuda:0", use_graphs: bool = True, fuse_decode: bool = True,
-                    fuse_prefill: bool = True) -> "Engine":
+                    fuse_prefill: bool = True, weight_bits: int = 16, cache_bits: int = 16) -> "Engine":
         dev = _require_gpu(device)
         config = load_config(folder)
         model = Model(config.to_spec())
+        model.check_bits(weight_bits, cache_bits)                         # before a large file is read
         kernel_build.prefetch(model.kernel_modules(_DTYPES[dtype]))       # in the background, while the weights are read
         tensors = load_tensors(folder, model.weight_specs(), dev, _DTYPES[dtype] == torch.float32)
-        return cls(config, tensors, dtype, max_tokens, max_seqs, device, use_graphs, fuse_decode, fuse_prefill)
+        return cls(config, tensors, dtype, max_tokens, max_seqs, device, use_graphs, fuse_decode, fuse_prefill, weight_bits, cache_bits)
 
     @classmethod
     def from_config(cls, config, seed: int = 0, dtype="bfloat16", max_tokens: int = 4096,
                     max_seqs: int | None = None, device="cuda:0", std: float = 0.02,
                     norm_std: float = 0.0, use_graphs: bool = True, fuse_decode: bool = True,
-                    fuse_prefill: bool = True) -> "Engine":
+                    fuse_prefill: bool = True, weight_bits: int = 16, cache_bits: int = 16) -> "Engine":
         """Random weights drawn on the device (no file); the same generator rule as the folder writer."""
         dev = _require_gpu(device)
         model = Model(config.to_spec())
         tensors = random_tensors(model.weight_specs(), seed, std, norm_std, torch.bfloat16, device=dev)
         if _DTYPES[dtype] == torch.float32:
             tensors = {k: (v.float() if v.is_floating_point() else v) for k, v in tensors.items()}
-        return cls(config, tensors, dtype, max_tokens, max_seqs, device, use_graphs, fuse_decode, fuse_prefill)
+        return cls(config, tensors, dtype, max_tokens, max_seqs, device, use_graphs, fuse_decode, fuse_prefill, weight_bits, cache_bits)
 
     # ------------------------------------------------------------------ slots
     def acquire(self) -> int:

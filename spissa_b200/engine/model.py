@@ -11,7 +11,7 @@ import torch
 
 from ..config.spec import ModelSpec
 from ..parts import registry as part_registry
-from ..parts.base import Runtime
+from ..parts.base import FeedForward, Mixer, Runtime
 from .. import parts as _parts  # noqa: F401  (registers the built-in parts)
 from ..phases import phase, profiling
 from ..csrc import lib as K
@@ -51,7 +51,23 @@ class Model:
         self.host_steps = True         # a short prompt step's launch sequence as one call into C++ likewise
         self._host_step = False
 
-    def kernel_modules(self, act_dtype) -> list:
+    def check_bits(self, weight_bits: int, cache_bits: int) -> None:
+        """Refuses a number of bits that there is no form for, and a model with layers whose parts have none."""
+        for name, bits in (("weight_bits", weight_bits), ("cache_bits", cache_bits)):
+            if bits not in (4, 16):
+                raise ValueError(f"{name} is 16 (as they come) or 4, got {bits}")
+        for layer in self.layers:
+            for part in layer.children():
+                own = vars(type(part))               # (not inherited: a subclass has kernels of its own)
+                mixer = isinstance(part, Mixer)
+                if not mixer and not isinstance(part, FeedForward):
+                    continue
+                if weight_bits == 4 and not own.get("four_bit_weights"):
+                    raise ValueError(f"{self.spec.architecture}: {type(part).__name__} has no form with weights of four bits")
+                if cache_bits == 4 and mixer and not own.get("four_bit_cache"):
+                    raise ValueError(f"{self.spec.architecture}: {type(part).__name__} has no form with a cache of four bits")
+
+    def kernel_modules(self, act_dtype, rt=None) -> list:
         """The kernel libraries that steps of this model can need, for building them ahead of their first use (a guess
         costs processor time only: a library is still built when it is first asked for)."""
         own = []                                    # libraries that parts name themselves (``kernel_modules`` of a class)
@@ -66,6 +82,10 @@ class Model:
                 walk(c)
         for p in self.parts():
             walk(p)
+        if rt is not None and rt.weight_bits == 4:
+            own.append("q4")
+        if rt is not None and rt.cache_bits == 4:
+            own += ["kv4", "kv4_attention"]
         if act_dtype != torch.bfloat16:
             return ["generic", "tc_f32"] + own
         mods = ["generic", "gemv", "tc_gemm", "tc_mid", "tc_stream"] + own

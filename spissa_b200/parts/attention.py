@@ -22,7 +22,7 @@ import torch
 from ..cache.views import KVLayerView
 from ..csrc import lib as K
 from .base import KVCacheRequest, Mixer, WeightSpec
-from .linear import GEMV_TOKENS, Linear
+from .linear import GEMV_TOKENS, held_linear
 from .registry import build_part, register_part
 from ..phases import phase
 
@@ -51,6 +51,7 @@ TILED_TOKENS = 32          # 32-bit prompt steps of at least so many tokens take
 @register_part("mixer", "attention")
 class GQAAttention(Mixer):
     graph_safe = True
+    four_bit_weights = four_bit_cache = True
 
     def __init__(self, hidden_size: int, num_heads: int, num_kv_heads: int, head_dim: int,
                  position=None, window=None, shares_kv: bool = False, prefix: str = "", names: dict | None = None):
@@ -82,24 +83,34 @@ class GQAAttention(Mixer):
         return own + [WeightSpec(self.names["k"], (nkv * hd, H)), WeightSpec(self.names["v"], (nkv * hd, H))]
 
     def cache_request(self):
-        return KVCacheRequest(self.num_kv_heads, self.head_dim, self.window)
+        bits = self.rt.cache_bits if self.rt is not None else 16
+        if bits == 4 and (self.head_dim not in K.KV4_HEAD_SIZES or self._rotated() % 8):
+            raise ValueError(f"{self.prefix}: a four-bit cache takes heads of {', '.join(map(str, K.KV4_HEAD_SIZES))} of which a multiple of 8 "
+                             f"dims is rotated, got {self.head_dim} and {self._rotated()}")
+        return KVCacheRequest(self.num_kv_heads, self.head_dim, self.window, bits=bits)
+
+    def _rotated(self) -> int:
+        return self.position.rotary_dim if self.position is not None and hasattr(self.position, "rotary") else 0
 
     def bind(self, tensors, rt):
         super().bind(tensors, rt)
         q = tensors[self.names["q"]]
-        self.q_only = Linear(q)
+        shared = rt.weight_bits == 4 and not self.shares_kv and q.shape[0] % 16 == 0        # q's rows are whole tiles of the packed q, k, v
+        self.q_only = None if shared else held_linear(q, rt)
         if not self.shares_kv:
             k, v = tensors[self.names["k"]], tensors[self.names["v"]]
             if not (q.dtype == k.dtype == v.dtype):
                 raise ValueError(f"{self.prefix}: q, k and v projections must share a storage type")
-            self.qkv = Linear(torch.cat([q, k, v], dim=0))
-        self.o = Linear(tensors[self.names["o"]])
+            self.qkv = held_linear(torch.cat([q, k, v], dim=0), rt)
+            if shared:
+                self.q_only = self.qkv.first_rows(q.shape[0])
+        self.o = held_linear(tensors[self.names["o"]], rt)
         # arrival counters of the split-key decode attention; the kernel returns them to zero
         self.counters = torch.zeros(4096, dtype=torch.int32, device=rt.device)
 
     def fused_fields(self):
         rotary = self.position is not None and hasattr(self.position, "rotary")
-        if self.shares_kv or self.window or not rotary or self.qkv is None:
+        if self.shares_kv or self.window or not rotary or self.qkv is None or self.rt.weight_bits != 16 or self.rt.cache_bits != 16:
             return None
         inv_freq, rd = self.position.rotary()
         if rd != self.head_dim or self.qkv.weight.dtype != torch.bfloat16 or self.o.weight.dtype != torch.bfloat16:
@@ -120,8 +131,8 @@ class GQAAttention(Mixer):
         if rotary:
             inv_freq, rd = self.position.rotary()
         q = torch.empty(T, nh * hd, dtype=self.rt.act_dtype, device=x.device)
-        w = self.qkv.weight if writes else None
-        if (writes and rotary and rd == hd and hd % 16 == 0 and T <= GEMV_TOKENS and q.dtype == torch.bfloat16
+        w = self.qkv.weight if writes and self.rt.weight_bits == 16 else None
+        if (w is not None and rotary and rd == hd and hd % 16 == 0 and T <= GEMV_TOKENS and q.dtype == torch.bfloat16
                 and cache.k_pool.dtype == torch.bfloat16 and K.gemv_supported(x, w)):
             # a few tokens: one kernel does the QKV product, the rotation and the cache write
             with phase("qkv_projection+rotary+kv_append_ms"):
@@ -137,7 +148,10 @@ class GQAAttention(Mixer):
             with phase("rotary+kv_append_ms"):
                 if self.position is not None and not rotary:
                     self.position.apply(qkv, step, nh, nkv, hd)
-                K.rope_kv_write(qkv, q, cache.k_pool, cache.v_pool, cache, inv_freq, nh, nkv, hd, rd, write_kv=writes)
+                if getattr(cache, "bits", 16) == 4:
+                    K.kv4_store(qkv, q, cache.k_pool, cache, inv_freq, nh, nkv, hd, rd, write_kv=writes)
+                else:
+                    K.rope_kv_write(qkv, q, cache.k_pool, cache.v_pool, cache, inv_freq, nh, nkv, hd, rd, write_kv=writes)
         with phase("attention_ms"):
             ctx = self.attend(q, step, cache)
         with phase("o_projection+attention_residual_ms"):

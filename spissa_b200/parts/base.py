@@ -45,6 +45,8 @@ class KVCacheRequest:
     ``head_dim`` is the size of a key row per kv head, ``v_head_dim`` that of a value row when it differs.
     ``keep_first``: with a window, the first ``keep_first`` positions stay visible to every later query, so the pages
     that hold them are never handed back while the sequence lives.
+    ``bits``: 4 asks for pages that hold keys and values in four bits with a scale and a zero for every 32 numbers
+    (csrc/q4.cuh): one pool of bytes, which is the view's ``k_pool`` and ``v_pool``.
     ``keys_only``: a position has ONE row, which its readers take as key and as value (a cached latent): no value pool
     is allocated and the view's ``v_pool`` is its ``k_pool``.
     """
@@ -54,6 +56,7 @@ class KVCacheRequest:
     v_head_dim: Optional[int] = None
     keep_first: int = 0
     keys_only: bool = False
+    bits: int = 16
 
 
 @dataclass(frozen=True)
@@ -80,11 +83,15 @@ class Runtime:
     """What the engine tells every part once: where and in which precision it runs.
 
     ``act_dtype`` is the storage type of activations between kernels and of the
-    cache: bfloat16 in the serving mode, float32 in the true 32-bit mode.
+    cache: bfloat16 in the serving mode, float32 in the true 32-bit mode. ``weight_bits`` and
+    ``cache_bits`` of 4 ask the parts that say they can (``four_bit_weights``, ``four_bit_cache``
+    of their own class) to hold their matrices, and keys and values, in four bits.
     """
     device: torch.device
     act_dtype: torch.dtype
     page_size: int = 64
+    weight_bits: int = 16
+    cache_bits: int = 16
 
     @property
     def full_precision(self) -> bool:

@@ -164,6 +164,15 @@ class Linear4:
         self.group = int(group)
         self.codes, self.scales = K.q4_pack(weight.contiguous(), self.group)
 
+    def first_rows(self, n: int) -> "Linear4":
+        """The product with the first ``n`` rows of the weight (a multiple of 16: the codes of whole tiles), sharing its codes."""
+        if n <= 0 or n % 16 or n > self.out_features:
+            raise ValueError(f"rows of a four-bit weight are taken in tiles of 16, got {n} of {self.out_features}")
+        part = Linear4.__new__(Linear4)
+        part.out_features, part.in_features, part.group = n, self.in_features, self.group
+        part.codes, part.scales = self.codes[:n // 16], self.scales[:n // 16]
+        return part
+
     def unpacked(self, dtype=torch.bfloat16) -> torch.Tensor:
         w = torch.empty(self.out_features, self.in_features, dtype=dtype, device=self.codes.device)
         K.q4_unpack(self.codes, self.scales, w, self.group)
@@ -215,6 +224,20 @@ class GatedLinear4:
         elif M:
             return self.unpacked(x.dtype)(x, act_dtype)
         return out
+
+
+def held_linear(weight: torch.Tensor, rt):
+    """A linear operator that holds its weight in as many bits as the runtime asks for."""
+    return Linear4(weight, group_of(weight)) if rt.weight_bits == 4 else Linear(weight)
+
+
+def held_gated(gate: torch.Tensor, up: torch.Tensor, act: int, mult: float, rt):
+    return GatedLinear4(gate, up, act, mult, group_of(gate)) if rt.weight_bits == 4 else GatedLinear(gate, up, act, mult)
+
+
+def group_of(weight: torch.Tensor) -> int:
+    """Columns that share a scale: 64 (4.25 bits a number), 32 where the rows are no multiple of that."""
+    return 64 if weight.shape[1] % 64 == 0 else 32
 
 
 _ROWS = (torch.bfloat16, torch.float32)

@@ -39,7 +39,7 @@ import torch
 
 from ..csrc import lib as K
 from .base import FeedForward, WeightSpec
-from .linear import GatedLinear, Linear
+from .linear import GatedLinear, Linear, held_gated, held_linear
 from .registry import build_part, register_part
 from ..phases import phase
 
@@ -47,6 +47,7 @@ from ..phases import phase
 @register_part("ffn", "swiglu")
 class SwiGLU(FeedForward):
     graph_safe = True
+    four_bit_weights = True
     act = K.ACT_SILU
 
     def __init__(self, hidden_size: int, intermediate_size: int, prefix: str = "", names: dict | None = None,
@@ -69,11 +70,13 @@ class SwiGLU(FeedForward):
         g, u = tensors[self.names["gate"]], tensors[self.names["up"]]
         if g.dtype != u.dtype:
             raise ValueError(f"{self.prefix}: gate and up projections must share a storage type")
-        self.gate_up = GatedLinear(g, u, self.act, self.out_scale)
-        self.down = Linear(tensors[self.names["down"]])
+        self.gate_up = held_gated(g, u, self.act, self.out_scale, rt)
+        self.down = held_linear(tensors[self.names["down"]], rt)
 
     def fused_fields(self):
         gu = self.gate_up
+        if self.rt is not None and self.rt.weight_bits != 16:
+            return None                          # the fused kernels read bfloat16 weights
         if self.act != K.ACT_SILU or self.out_scale != 1.0 or gu is None or not gu.block or gu.weight.dtype != torch.bfloat16 or self.down.weight.dtype != torch.bfloat16:
             return None
         return dict(kind="swiglu", gate_up=gu.weight, pair=gu.block, down=self.down.weight,
@@ -94,6 +97,7 @@ class SwiGLU(FeedForward):
 @register_part("ffn", "geglu")
 class GeGLU(SwiGLU):
     """The gated feed-forward with the tanh form of gelu on the gate."""
+    four_bit_weights = True
     act = K.ACT_GELU
 
 
