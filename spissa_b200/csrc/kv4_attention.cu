@@ -110,7 +110,7 @@ __device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
     for (int i = 0; i < 8; ++i) v[i] = finite_or_nan(v[i]);
 }
 
-// scale (group i of a row's half words) and zero as numbers; the zero through the place of ones of 2^23
+// scale (group i of a row's half words) and zero as numbers; the zero from the last place of 2^23
 __device__ __forceinline__ float scale_at(const uint32_t* m, int i) {
     return __uint_as_float(i & 1 ? m[i >> 1] & 0xfff00000u : (m[i >> 1] << 16) & 0xfff00000u);
 }
@@ -122,6 +122,7 @@ template <typename TQ, int NG, int NT>
 __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 2)
 attend_kernel(const Args a) {
     constexpr int HD = 32 * NG, PARTS = sizeof(TQ) == 4 ? 2 : 1, COLS = 8 * NT, TILE = kv4_tile_bytes(HD), MW = (NG + 1) / 2;
+    constexpr int PP = NT == 1 ? 2 : 1;
     constexpr bool Q_HELD = NT == 1 && PARTS == 1;                   // the queries' operands in registers, else in shared memory
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES];
@@ -217,54 +218,62 @@ attend_kernel(const Args a) {
     }
     if (!Q_HELD) __syncthreads();
 
-    float O[NT][NG][2][4], zs[NT][NG][2], sum[NT][2], ref[NT][2], top[NT][2];      // top: the score that the reference was made for
+    // top: the score (log2, rounded up) that a column's reference was made for; limit: how far a raw score may go under it
+    float O[NT][NG][2][4], Z[PARTS == 1 ? NT : 1][NG][4], sum[NT][2], ref[NT][2], top[NT][2], limit[NT][2];
     uint32_t poison[NT];
-    float s_top = 0.0f;                                              // the scale that the references were made for
+    uint32_t s_bits = 0;                                             // the largest scale the references were made for, twice, zeros of 15
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         poison[n] = 0;
 #pragma unroll
         for (int i = 0; i < NG; ++i) {
-            zs[n][i][0] = zs[n][i][1] = 0.0f;
+            if (PARTS == 1) Z[PARTS == 1 ? n : 0][i][0] = Z[PARTS == 1 ? n : 0][i][1] = Z[PARTS == 1 ? n : 0][i][2] = Z[PARTS == 1 ? n : 0][i][3] = 0.0f;
 #pragma unroll
             for (int h = 0; h < 2; ++h) O[n][i][h][0] = O[n][i][h][1] = O[n][i][h][2] = O[n][i][h][3] = 0.0f;
         }
 #pragma unroll
-        for (int e = 0; e < 2; ++e) { sum[n][e] = 0.0f; ref[n][e] = 0.0f; top[n][e] = -INFINITY; }
+        for (int e = 0; e < 2; ++e) { sum[n][e] = 0.0f; ref[n][e] = 0.0f; top[n][e] = limit[n][e] = -INFINITY; }
     }
 
-    for (int it = 0; it < n_pages; ++it) {
-        const int s = it % STAGES, page_pos = (page0 + it) * KV4_PAGE;
-        // the stage that every warp had done with a page ago gets the next page
-        if (threadIdx.x == 0 && it >= 1 && it - 1 + STAGES < n_pages) {
-            if (mbar_wait_flag(smem_u32(&empty[(it - 1) % STAGES]), ((it - 1) / STAGES) & 1, a.status, 141, &failed)) fetch(it - 1 + STAGES);
-        }
-        __syncwarp();
-        mbar_wait_flag(smem_u32(&full[s]), (it / STAGES) & 1, a.status, 142, &failed);
-        const uint32_t at = ring + s * TILE;
-        const int r0 = warp * 16 + g;                                // rows of the page's keys as they lie: this lane's are r0 and r0 + 8
-        const int key = page_pos + warp * 16 + (g & 1) * 4 + (g >> 1);        // their positions: this and 8 on
-        const bool partly = page_pos + KV4_PAGE - 1 > first_pos || (a.window && page_pos < last_pos + 1 - a.window);
-
-        // scores of 16 keys: rows g and g + 8, columns 2 t and 2 t + 1
-        float x[NT][4];
+    // PP pages a turn: two where registers allow it, so that one's scores are under way beside the other's
+    for (int it = 0; it < n_pages; it += PP) {
+        // the stages that every warp had done with a turn ago get the next pages
+        if (threadIdx.x == 0 && it > 0)
 #pragma unroll
-        for (int n = 0; n < NT; ++n) x[n][0] = x[n][1] = x[n][2] = x[n][3] = 0.0f;
-        {
-            uint32_t k0[NG], k1[NG], m0[MW], m1[MW];
+            for (int j = 0; j < PP; ++j) {
+                const int done = it - PP + j;
+                if (done + STAGES < n_pages && mbar_wait_flag(smem_u32(&empty[done % STAGES]), (done / STAGES) & 1, a.status, 141, &failed)) fetch(done + STAGES);
+            }
+        __syncwarp();
+        float x[PP][NT][4];
+        uint32_t m0[PP][MW], m1[PP][MW];                             // the values' scales of this lane's two keys of a page
+#pragma unroll
+        for (int j = 0; j < PP; ++j) {
+            const bool here = it + j < n_pages;                      // (the last turn may lack a page: nobody sees its keys)
+            if (here) mbar_wait_flag(smem_u32(&full[(it + j) % STAGES]), ((it + j) / STAGES) & 1, a.status, 142, &failed);
+            const int page_pos = (page0 + it + j) * KV4_PAGE;
+            const uint32_t at = ring + ((it + j) % STAGES) * TILE;
+            const int r0 = warp * 16 + g;                            // rows of the page's keys as they lie: this lane's are r0 and r0 + 8
+            const int p0 = warp * 16 + (g & 1) * 4 + (g >> 1), key = page_pos + p0;        // their positions: this and 8 on
+            // scores of 16 keys: rows g and g + 8, columns 2 t and 2 t + 1
+#pragma unroll
+            for (int n = 0; n < NT; ++n) x[j][n][0] = x[j][n][1] = x[j][n][2] = x[j][n][3] = 0.0f;
+            uint32_t k0[NG], k1[NG], km0[MW], km1[MW];
             lds_words<NG>(at + r0 * (HD / 2) + t * (NG * 4), k0);
             lds_words<NG>(at + (r0 + 8) * (HD / 2) + t * (NG * 4), k1);
-            lds_halves<NG>(at + kv4_k_meta(HD) + r0 * (NG * 2), m0);
-            lds_halves<NG>(at + kv4_k_meta(HD) + (r0 + 8) * (NG * 2), m1);
+            lds_halves<NG>(at + kv4_k_meta(HD) + r0 * (NG * 2), km0);
+            lds_halves<NG>(at + kv4_k_meta(HD) + (r0 + 8) * (NG * 2), km1);
+            lds_halves<NG>(at + kv4_v_meta(HD) + p0 * (NG * 2), m0[j]);
+            lds_halves<NG>(at + kv4_v_meta(HD) + (p0 + 8) * (NG * 2), m1[j]);
 #pragma unroll
             for (int i = 0; i < NG; ++i) {
-                const float s0 = scale_at(m0, i), s1 = scale_at(m1, i), z0 = zero_at(m0, i), z1 = zero_at(m1, i);
+                const float s0 = scale_at(km0, i), s1 = scale_at(km1, i), z0 = zero_at(km0, i), z1 = zero_at(km1, i);
                 const uint32_t u0 = k0[i], u1 = k1[i], w0 = u0 >> 8, w1 = u1 >> 8;
                 uint32_t c[8] = {u0 & 0x000f000fu, u1 & 0x000f000fu, u0 & 0x00f000f0u, u1 & 0x00f000f0u, w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u};
                 if (PARTS == 2) {
-                    const uint32_t y0 = ((m0[i >> 1] >> (16 * (i & 1))) & 15u) * 0x10001u, y1 = ((m1[i >> 1] >> (16 * (i & 1))) & 15u) * 0x10001u;
+                    const uint32_t y0 = ((km0[i >> 1] >> (16 * (i & 1))) & 15u) * 0x10001u, y1 = ((km1[i >> 1] >> (16 * (i & 1))) & 15u) * 0x10001u;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) c[j] = q4_less(c[j], (j & 1 ? y1 : y0) << (j & 2 ? 4 : 0));
+                    for (int k = 0; k < 8; ++k) c[k] = q4_less(c[k], (k & 1 ? y1 : y0) << (k & 2 ? 4 : 0));
                 }
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
@@ -277,156 +286,161 @@ attend_kernel(const Args a) {
                         mma_f16(acc, c[0], c[1], c[2], c[3], qv.x, qv.y);
                         mma_f16(acc, c[4], c[5], c[6], c[7], qv.z, qv.w);
                     }
+                    float (&y)[4] = x[j][n];
                     if (PARTS == 2) {
-                        x[n][0] = fmaf(s0, acc[0], x[n][0]);
-                        x[n][1] = fmaf(s0, acc[1], x[n][1]);
-                        x[n][2] = fmaf(s1, acc[2], x[n][2]);
-                        x[n][3] = fmaf(s1, acc[3], x[n][3]);
+                        y[0] = fmaf(s0, acc[0], y[0]);
+                        y[1] = fmaf(s0, acc[1], y[1]);
+                        y[2] = fmaf(s1, acc[2], y[2]);
+                        y[3] = fmaf(s1, acc[3], y[3]);
                         continue;
                     }
-                    x[n][0] = fmaf(s0, fmaf(z0, qs[n][i][0], acc[0]), x[n][0]);
-                    x[n][1] = fmaf(s0, fmaf(z0, qs[n][i][1], acc[1]), x[n][1]);
-                    x[n][2] = fmaf(s1, fmaf(z1, qs[n][i][0], acc[2]), x[n][2]);
-                    x[n][3] = fmaf(s1, fmaf(z1, qs[n][i][1], acc[3]), x[n][3]);
+                    y[0] = fmaf(s0, fmaf(z0, qs[n][i][0], acc[0]), y[0]);
+                    y[1] = fmaf(s0, fmaf(z0, qs[n][i][1], acc[1]), y[1]);
+                    y[2] = fmaf(s1, fmaf(z1, qs[n][i][0], acc[2]), y[2]);
+                    y[3] = fmaf(s1, fmaf(z1, qs[n][i][1], acc[3]), y[3]);
                 }
             }
-        }
-        uint32_t m0[MW], m1[MW];                                     // the values' scales of the same two keys
-        {
-            const int p0 = warp * 16 + (g & 1) * 4 + (g >> 1);
-            lds_halves<NG>(at + kv4_v_meta(HD) + p0 * (NG * 2), m0);
-            lds_halves<NG>(at + kv4_v_meta(HD) + (p0 + 8) * (NG * 2), m1);
-        }
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                x[n][e] *= unit[n][e & 1];
-                if (partly) {
-                    const int p = pos[n][e & 1], j = key + (e & 2) * 4;
-                    if (j > p || (a.window && j <= p - a.window)) x[n][e] = -INFINITY;
-                }
-            }
-        if (partly) {                                                // what nobody sees may be anything
-#pragma unroll
-            for (int i = 0; i < MW; ++i) {
-                if (key > last_pos || key < lowest) m0[i] = 0;
-                if (key + 8 > last_pos || key + 8 < lowest) m1[i] = 0;
-            }
-        }
-        // do the references hold?
-        uint32_t most = 0;
-#pragma unroll
-        for (int i = 0; i < MW; ++i) most = __vmaxu2(most, __vmaxu2(m0[i], m1[i]));
-        most = max(most & 0xffffu, most >> 16);
-        bool moves = __uint_as_float((most & 0xfff0u) << 16) > s_top || (most & 0x7f80u) == 0x7f80u;
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) moves |= x[n][e] > top[n][e & 1] + STEP;
-        if (__any_sync(0xffffffffu, moves)) {
-            // scales that are not numbers: noted for the columns that see their keys, and taken as zero
-#pragma unroll
-            for (int i = 0; i < NG; ++i) {
-                const int sh = 16 * (i & 1);
-                const bool bad0 = ((m0[i >> 1] >> sh) & 0x7f80u) == 0x7f80u, bad1 = ((m1[i >> 1] >> sh) & 0x7f80u) == 0x7f80u;
+            if (!here || page_pos + KV4_PAGE - 1 > first_pos || (a.window && page_pos < last_pos + 1 - a.window)) {       // not all of it is seen by all
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e)
-                        if ((bad0 && x[n][e] != -INFINITY) || (bad1 && x[n][2 + e] != -INFINITY)) poison[n] |= 1u << (2 * i + e);
-                if (bad0) m0[i >> 1] &= ~(0xffffu << sh);
-                if (bad1) m1[i >> 1] &= ~(0xffffu << sh);
+                    for (int e = 0; e < 4; ++e) {
+                        const int p = pos[n][e & 1], k = key + (e & 2) * 4;
+                        if (!here || k > p || (a.window && k <= p - a.window)) x[j][n][e] = -INFINITY;
+                    }
+#pragma unroll
+                for (int i = 0; i < MW; ++i) {                       // what nobody sees may be anything
+                    if (!here || key > last_pos || key < lowest) m0[j][i] = 0;
+                    if (!here || key + 8 > last_pos || key + 8 < lowest) m1[j][i] = 0;
+                }
             }
+        }
+        // do the references hold?
+        uint32_t most = s_bits;
+        bool moves = false;
+#pragma unroll
+        for (int j = 0; j < PP; ++j) {
+#pragma unroll
+            for (int i = 0; i < MW; ++i) most = __vmaxu2(most, __vmaxu2(m0[j][i], m1[j][i]));
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) moves |= x[j][n][e] > limit[n][e & 1];
+        }
+        if (__any_sync(0xffffffffu, moves || most != s_bits)) {
+            // scales that are not numbers: noted for the columns that see their keys, and taken as zero
             most = 0;
 #pragma unroll
-            for (int i = 0; i < MW; ++i) most = __vmaxu2(most, __vmaxu2(m0[i], m1[i]));
-            most = max(most & 0xffffu, most >> 16);
-            const uint32_t all = __reduce_max_sync(0xffffffffu, most & 0xfff0u);
-            s_top = fmaxf(s_top, __uint_as_float(all << 16));
+            for (int j = 0; j < PP; ++j) {
+#pragma unroll
+                for (int i = 0; i < NG; ++i) {
+                    const int sh = 16 * (i & 1);
+                    const bool bad0 = ((m0[j][i >> 1] >> sh) & 0x7f80u) == 0x7f80u, bad1 = ((m1[j][i >> 1] >> sh) & 0x7f80u) == 0x7f80u;
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+                            if ((bad0 && x[j][n][e] != -INFINITY) || (bad1 && x[j][n][2 + e] != -INFINITY)) poison[n] |= 1u << (2 * i + e);
+                    if (bad0) m0[j][i >> 1] &= ~(0xffffu << sh);
+                    if (bad1) m1[j][i >> 1] &= ~(0xffffu << sh);
+                }
+#pragma unroll
+                for (int i = 0; i < MW; ++i) most = __vmaxu2(most, __vmaxu2(m0[j][i], m1[j][i]));
+            }
+            most = max(most & 0xffffu, most >> 16) | 15u;             // (with every zero: what is compared is the whole half word)
+            s_bits = max(s_bits & 0xffffu, __reduce_max_sync(0xffffffffu, most)) * 0x10001u;
+            const float s_top = __uint_as_float((s_bits & 0xfff0u) << 16);
             const float es = s_top > 0.0f ? (float)((int)(__float_as_uint(s_top) >> 23) - 126) : 0.0f;         // s_top < 2^es
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 float f[2];
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    float big = fmaxf(x[n][e], x[n][2 + e]);
+                    float big = fmaxf(x[0][n][e], x[0][n][2 + e]);
+#pragma unroll
+                    for (int j = 1; j < PP; ++j) big = fmaxf(big, fmaxf(x[j][n][e], x[j][n][2 + e]));
                     big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 4));
                     big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 8));
                     big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 16));
                     const bool had = top[n][e] != -INFINITY;
-                    if (big > top[n][e] + STEP) top[n][e] = big;
+                    if (big > limit[n][e]) {
+                        top[n][e] = ceilf(big * unit[n][e]);
+                        limit[n][e] = (top[n][e] + STEP) / unit[n][e];
+                    }
                     const float was = ref[n][e];
                     // p s <= 2^(STEP + top − ref + es) = 2^15; whole steps, so that the factors are powers of two
-                    ref[n][e] = top[n][e] != -INFINITY ? ceilf(top[n][e]) + es + STEP - 15.0f : 0.0f;
+                    ref[n][e] = top[n][e] != -INFINITY ? top[n][e] + es + STEP - 15.0f : 0.0f;
                     f[e] = had ? ex2(was - ref[n][e]) : 1.0f;
                     sum[n][e] *= f[e];
                 }
 #pragma unroll
                 for (int i = 0; i < NG; ++i) {
-                    zs[n][i][0] *= f[0];
-                    zs[n][i][1] *= f[1];
 #pragma unroll
                     for (int h = 0; h < 2; ++h) { O[n][i][h][0] *= f[0]; O[n][i][h][1] *= f[1]; O[n][i][h][2] *= f[0]; O[n][i][h][3] *= f[1]; }
+                    if (PARTS == 1) { float (&z)[4] = Z[PARTS == 1 ? n : 0][i]; z[0] *= f[0]; z[1] *= f[1]; z[2] *= f[0]; z[3] *= f[1]; }
                 }
             }
         }
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
+        for (int j = 0; j < PP; ++j) {
+            const uint32_t at = ring + ((it + j) % STAGES) * TILE;
+            float (&y)[NT][4] = x[j];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[n][e] = ex2(x[n][e] - ref[n][e & 1]);
-            sum[n][0] += x[n][0] + x[n][2];
-            sum[n][1] += x[n][1] + x[n][3];
-        }
-        // the output of 16 keys
-        {
-            uint32_t v[4][MW], mz[PARTS == 2 ? 4 : 1][MW];
+            for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[n][e] = ex2(fmaf(y[n][e], unit[n][e & 1], -ref[n][e & 1]));
+                sum[n][0] += y[n][0] + y[n][2];
+                sum[n][1] += y[n][1] + y[n][3];
+            }
+            // the output of 16 keys
+            uint32_t v[4][MW], mz[4][MW];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const int p = warp * 16 + 4 * k + t, sw = HD == 128 ? (p & 2) << 4 : 0;
                 lds_halves<NG>(at + kv4_v_codes(HD) + p * (HD / 2) + ((g * NG * 2) ^ sw), v[k]);
-                if (PARTS == 2) lds_halves<NG>(at + kv4_v_meta(HD) + p * (NG * 2), mz[PARTS == 2 ? k : 0]);
+                lds_halves<NG>(at + kv4_v_meta(HD) + p * (NG * 2), mz[k]);
             }
 #pragma unroll
             for (int i = 0; i < NG; ++i) {
-                const float s0 = scale_at(m0, i), s1 = scale_at(m1, i), z0 = zero_at(m0, i), z1 = zero_at(m1, i);
-                const uint32_t u0 = __byte_perm(v[0][i >> 1], v[1][i >> 1], i & 1 ? 0x7632 : 0x5410), u1 = __byte_perm(v[2][i >> 1], v[3][i >> 1], i & 1 ? 0x7632 : 0x5410);
-                const uint32_t w0 = u0 >> 8, w1 = u1 >> 8;      // keys t, 4 + t and 8 + t, 12 + t side by side
+                const float s0 = scale_at(m0[j], i), s1 = scale_at(m1[j], i);
+                const int half = i & 1 ? 0x7632 : 0x5410;
+                // keys t, 4 + t and 8 + t, 12 + t side by side; their zeros likewise
+                const uint32_t u0 = __byte_perm(v[0][i >> 1], v[1][i >> 1], half), u1 = __byte_perm(v[2][i >> 1], v[3][i >> 1], half);
+                const uint32_t y0 = __byte_perm(mz[0][i >> 1], mz[1][i >> 1], half) & 0x000f000fu, y1 = __byte_perm(mz[2][i >> 1], mz[3][i >> 1], half) & 0x000f000fu;
+                const uint32_t w0 = u0 >> 8, w1 = u1 >> 8;
                 uint32_t c[8] = {u0 & 0x000f000fu, u0 & 0x00f000f0u, u1 & 0x000f000fu, u1 & 0x00f000f0u, w0 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x000f000fu, w1 & 0x00f000f0u};
-                if (PARTS == 2) {
-                    const uint32_t y0 = __byte_perm(mz[0][i >> 1], mz[PARTS == 2 ? 1 : 0][i >> 1], i & 1 ? 0x7632 : 0x5410) & 0x000f000fu;
-                    const uint32_t y1 = __byte_perm(mz[PARTS == 2 ? 2 : 0][i >> 1], mz[PARTS == 2 ? 3 : 0][i >> 1], i & 1 ? 0x7632 : 0x5410) & 0x000f000fu;
+                if (PARTS == 2)
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) c[j] = q4_less(c[j], (j & 2 ? y1 : y0) << (j & 1 ? 4 : 0));
-                }
+                    for (int k = 0; k < 8; ++k) c[k] = q4_less(c[k], (k & 2 ? y1 : y0) << (k & 1 ? 4 : 0));
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    const float p0 = x[n][0] * s0, p1 = x[n][1] * s0, p2 = x[n][2] * s1, p3 = x[n][3] * s1;
+                    const float p0 = y[n][0] * s0, p1 = y[n][1] * s0, p2 = y[n][2] * s1, p3 = y[n][3] * s1;
                     const uint32_t h0 = half2_of(p0, p1), h1 = half2_of(p2, p3), b0 = transposed(h0), b1 = transposed(h1);
-                    const float2 f0 = __half22float2(*(const __half2*)&h0), f1 = __half22float2(*(const __half2*)&h1);
                     if (PARTS == 2) {
                         // sums of a page of their own, added in 32 bits: the tensor cores' own additions cut instead of rounding
+                        const float2 f0 = __half22float2(*(const __half2*)&h0), f1 = __half22float2(*(const __half2*)&h1);
                         const uint32_t l0 = transposed(half2_of(p0 - f0.x, p1 - f0.y)), l1 = transposed(half2_of(p2 - f1.x, p3 - f1.y));
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            float y[4] = {0.f, 0.f, 0.f, 0.f};
-                            mma_f16(y, c[4 * h], c[4 * h + 1], c[4 * h + 2], c[4 * h + 3], l0, l1);
-                            mma_f16(y, c[4 * h], c[4 * h + 1], c[4 * h + 2], c[4 * h + 3], b0, b1);
+                            float o[4] = {0.f, 0.f, 0.f, 0.f};
+                            mma_f16(o, c[4 * h], c[4 * h + 1], c[4 * h + 2], c[4 * h + 3], l0, l1);
+                            mma_f16(o, c[4 * h], c[4 * h + 1], c[4 * h + 2], c[4 * h + 3], b0, b1);
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) O[n][i][h][e] += y[e];
+                            for (int e = 0; e < 4; ++e) O[n][i][h][e] += o[e];
                         }
                         continue;
                     }
                     mma_f16(O[n][i][0], c[0], c[1], c[2], c[3], b0, b1);
                     mma_f16(O[n][i][1], c[4], c[5], c[6], c[7], b0, b1);
-                    // (the zeros are taken off with the same rounded numbers, so that a value of zero adds exactly nothing)
-                    zs[n][i][0] = fmaf(f0.x, z0, fmaf(f1.x, z1, zs[n][i][0]));
-                    zs[n][i][1] = fmaf(f0.y, z0, fmaf(f1.y, z1, zs[n][i][1]));
+                    mma_f16(Z[PARTS == 1 ? n : 0][i], y0, y0, y1, y1, b0, b1);        // Σ p s z with the same rounded numbers, in every row
                 }
             }
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&empty[s]));
+        if (lane == 0)
+#pragma unroll
+            for (int j = 0; j < PP; ++j)
+                if (it + j < n_pages) mbar_arrive(smem_u32(&empty[(it + j) % STAGES]));
     }
 
     // each warp's sums over its lanes; then the warps', in their order, in shared memory (where the pages were)
@@ -437,8 +451,6 @@ attend_kernel(const Args a) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 sum[n][e] += __shfl_xor_sync(0xffffffffu, sum[n][e], o);
-#pragma unroll
-                for (int i = 0; i < NG; ++i) zs[n][i][e] += __shfl_xor_sync(0xffffffffu, zs[n][i][e], o);
             }
             poison[n] |= __shfl_xor_sync(0xffffffffu, poison[n], o);
         }
@@ -467,7 +479,8 @@ attend_kernel(const Args a) {
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
                             float2* to = (float2*)(acc + c * HD + 32 * i + 4 * g + 2 * h);
-                            float2 v = make_float2(fmaf(O[n][i][h][e], PARTS == 2 ? 1.0f : 16777216.0f, -zs[n][i][e]) * f, fmaf(O[n][i][h][2 + e], PARTS == 2 ? 0.0625f : 1048576.0f, -zs[n][i][e]) * f);
+                            const float z = PARTS == 1 ? Z[PARTS == 1 ? n : 0][i][e] : 0.0f, up = PARTS == 1 ? 16777216.0f : 1.0f;
+                            float2 v = make_float2((O[n][i][h][e] - z) * up * f, (O[n][i][h][2 + e] * 0.0625f - z) * up * f);
                             if (f == 0.0f) v = make_float2(0.0f, 0.0f);
                             if (poison[n] >> (2 * i + e) & 1) v.x = v.y = __int_as_float(0x7fc00000);
                             if (w > 0) { v.x += to->x; v.y += to->y; }
@@ -603,6 +616,7 @@ SP_API int sp_kv4_attend(const void* q, void* out, int dt, const void* pool, con
     if (nt != 1 && nt != 2 && nt != 4) SP_FAIL("kv4_attention: 8, 16 or 32 columns a CTA, got 8 x %d", nt);
     if (window < 0 || max_new <= 0 || (!seq_start && (max_new != 1 || T != n_seqs))) SP_FAIL("kv4_attention: window %d, %d tokens of %d sequences, at most %d of one", window, T, n_seqs, max_new);
     if (chunk_pages <= 0 || n_chunks <= 0 || n_chunks > 65535) SP_FAIL("kv4_attention: %d chunks of %d pages", n_chunks, chunk_pages);
+    if (!(scale > 0.0f) || scale > 1e30f) SP_FAIL("kv4_attention: a positive scale is wanted, got %g", scale);
     if (((uintptr_t)q & 15) || ((uintptr_t)pool & 15)) SP_FAIL("kv4_attention: queries and pages must start on 16-byte boundaries");
     if (sp_kv4_attend_scratch(T, nh, hd, n_chunks) > scratch_floats) SP_FAIL("kv4_attention: %lld floats of scratch are needed, got %lld", sp_kv4_attend_scratch(T, nh, hd, n_chunks), scratch_floats);
     const Args a{q, out, (const uint8_t*)pool, seq_start, positions, seq_row, page_table, sink, scratch, status,
