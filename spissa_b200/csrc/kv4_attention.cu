@@ -122,7 +122,7 @@ template <typename TQ, int NG, int NT>
 __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 2)
 attend_kernel(const Args a) {
     constexpr int HD = 32 * NG, PARTS = sizeof(TQ) == 4 ? 2 : 1, COLS = 8 * NT, TILE = kv4_tile_bytes(HD), MW = (NG + 1) / 2;
-    constexpr int PP = NT == 1 ? 2 : 1;
+    constexpr int PP = 1;
     constexpr bool Q_HELD = NT == 1 && PARTS == 1;                   // the queries' operands in registers, else in shared memory
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES];
@@ -138,6 +138,8 @@ attend_kernel(const Args a) {
     const int page0 = lowest / KV4_PAGE + chunk * a.chunk_pages, page1 = min(page0 + a.chunk_pages, last_pos / KV4_PAGE + 1);
     const int n_pages = max(0, page1 - page0), row = sp_checked_row(a.seq_row[seq], a.rg);
     const int* table = a.page_table + (size_t)row * a.max_pages;
+    constexpr int ROW = HD + 8;                                      // of the joined sums: neighbouring columns' rows lie in other banks
+    float* acc = (float*)smem;                                       // [warp][column][ROW]
     const uint32_t ring = smem_u32(smem), q_at = ring + STAGES * TILE;
 
     if (threadIdx.x == 0) {
@@ -150,13 +152,22 @@ attend_kernel(const Args a) {
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     __syncthreads();
-    auto fetch = [&](int i) {                                        // one thread
-        const int s = i % STAGES, page = sp_checked_page(table[sp_checked_entry(page0 + i, a.max_pages, a.rg)], a.rg);
+    // the first warp's lanes hold the numbers of 32 pages
+    int held = 0;
+    auto hold = [&](int i) { if (i + lane < n_pages) held = sp_checked_page(table[sp_checked_entry(page0 + i + lane, a.max_pages, a.rg)], a.rg); };
+    auto fetch = [&](int i, int page) {                              // one thread
+        const int s = i % STAGES;
         mbar_expect_tx(smem_u32(&full[s]), TILE);
         bulk_copy_g2s(ring + s * TILE, a.pool + ((size_t)page * a.nkv + kvh) * TILE, TILE, smem_u32(&full[s]));
     };
-    if (threadIdx.x == 0)
-        for (int i = 0; i < min(STAGES, n_pages); ++i) fetch(i);
+    if (warp == 0) {
+        hold(0);
+#pragma unroll
+        for (int i = 0; i < STAGES; ++i) {
+            const int page = __shfl_sync(0xffffffffu, held, i);
+            if (lane == 0 && i < n_pages) fetch(i, page);
+        }
+    }
 
     // The queries: lane (column g, dims 32 i + 8 t ..). Columns that are not there are zeros and see nothing.
     uint32_t qh[Q_HELD ? NG : 1][4];
@@ -219,7 +230,7 @@ attend_kernel(const Args a) {
     if (!Q_HELD) __syncthreads();
 
     // top: the score (log2, rounded up) that a column's reference was made for; limit: how far a raw score may go under it
-    float O[NT][NG][2][4], Z[PARTS == 1 ? NT : 1][NG][4], sum[NT][2], ref[NT][2], top[NT][2], limit[NT][2];
+    float O[NT][NG][2][4], zs[NT][NG][2], sum[NT][2], ref[NT][2], top[NT][2], limit[NT][2];
     uint32_t poison[NT];
     uint32_t s_bits = 0;                                             // the largest scale the references were made for, twice, zeros of 15
 #pragma unroll
@@ -227,7 +238,7 @@ attend_kernel(const Args a) {
         poison[n] = 0;
 #pragma unroll
         for (int i = 0; i < NG; ++i) {
-            if (PARTS == 1) Z[PARTS == 1 ? n : 0][i][0] = Z[PARTS == 1 ? n : 0][i][1] = Z[PARTS == 1 ? n : 0][i][2] = Z[PARTS == 1 ? n : 0][i][3] = 0.0f;
+            zs[n][i][0] = zs[n][i][1] = 0.0f;
 #pragma unroll
             for (int h = 0; h < 2; ++h) O[n][i][h][0] = O[n][i][h][1] = O[n][i][h][2] = O[n][i][h][3] = 0.0f;
         }
@@ -235,15 +246,14 @@ attend_kernel(const Args a) {
         for (int e = 0; e < 2; ++e) { sum[n][e] = 0.0f; ref[n][e] = 0.0f; top[n][e] = limit[n][e] = -INFINITY; }
     }
 
-    // PP pages a turn: two where registers allow it, so that one's scores are under way beside the other's
     for (int it = 0; it < n_pages; it += PP) {
-        // the stages that every warp had done with a turn ago get the next pages
-        if (threadIdx.x == 0 && it > 0)
-#pragma unroll
-            for (int j = 0; j < PP; ++j) {
-                const int done = it - PP + j;
-                if (done + STAGES < n_pages && mbar_wait_flag(smem_u32(&empty[done % STAGES]), (done / STAGES) & 1, a.status, 141, &failed)) fetch(done + STAGES);
-            }
+        // the stage that every warp had done with a page ago gets the next page
+        if (warp == 0 && it > 0 && it - 1 + STAGES < n_pages) {
+            const int i = it - 1 + STAGES;
+            if (i % 32 == 0) hold(i);
+            const int page = __shfl_sync(0xffffffffu, held, i % 32);
+            if (lane == 0 && mbar_wait_flag(smem_u32(&empty[(it - 1) % STAGES]), ((it - 1) / STAGES) & 1, a.status, 141, &failed)) fetch(i, page);
+        }
         __syncwarp();
         float x[PP][NT][4];
         uint32_t m0[PP][MW], m1[PP][MW];                             // the values' scales of this lane's two keys of a page
@@ -377,7 +387,8 @@ attend_kernel(const Args a) {
                 for (int i = 0; i < NG; ++i) {
 #pragma unroll
                     for (int h = 0; h < 2; ++h) { O[n][i][h][0] *= f[0]; O[n][i][h][1] *= f[1]; O[n][i][h][2] *= f[0]; O[n][i][h][3] *= f[1]; }
-                    if (PARTS == 1) { float (&z)[4] = Z[PARTS == 1 ? n : 0][i]; z[0] *= f[0]; z[1] *= f[1]; z[2] *= f[0]; z[3] *= f[1]; }
+                    zs[n][i][0] *= f[0];
+                    zs[n][i][1] *= f[1];
                 }
             }
         }
@@ -393,25 +404,27 @@ attend_kernel(const Args a) {
                 sum[n][1] += y[n][1] + y[n][3];
             }
             // the output of 16 keys
-            uint32_t v[4][MW], mz[4][MW];
+            uint32_t v[4][MW], mz[PARTS == 2 ? 4 : 1][MW];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const int p = warp * 16 + 4 * k + t, sw = HD == 128 ? (p & 2) << 4 : 0;
                 lds_halves<NG>(at + kv4_v_codes(HD) + p * (HD / 2) + ((g * NG * 2) ^ sw), v[k]);
-                lds_halves<NG>(at + kv4_v_meta(HD) + p * (NG * 2), mz[k]);
+                if (PARTS == 2) lds_halves<NG>(at + kv4_v_meta(HD) + p * (NG * 2), mz[PARTS == 2 ? k : 0]);
             }
 #pragma unroll
             for (int i = 0; i < NG; ++i) {
                 const float s0 = scale_at(m0[j], i), s1 = scale_at(m1[j], i);
                 const int half = i & 1 ? 0x7632 : 0x5410;
-                // keys t, 4 + t and 8 + t, 12 + t side by side; their zeros likewise
+                // keys t, 4 + t and 8 + t, 12 + t side by side
                 const uint32_t u0 = __byte_perm(v[0][i >> 1], v[1][i >> 1], half), u1 = __byte_perm(v[2][i >> 1], v[3][i >> 1], half);
-                const uint32_t y0 = __byte_perm(mz[0][i >> 1], mz[1][i >> 1], half) & 0x000f000fu, y1 = __byte_perm(mz[2][i >> 1], mz[3][i >> 1], half) & 0x000f000fu;
                 const uint32_t w0 = u0 >> 8, w1 = u1 >> 8;
                 uint32_t c[8] = {u0 & 0x000f000fu, u0 & 0x00f000f0u, u1 & 0x000f000fu, u1 & 0x00f000f0u, w0 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x000f000fu, w1 & 0x00f000f0u};
-                if (PARTS == 2)
+                if (PARTS == 2) {
+                    const uint32_t y0 = __byte_perm(mz[0][i >> 1], mz[PARTS == 2 ? 1 : 0][i >> 1], half) & 0x000f000fu;
+                    const uint32_t y1 = __byte_perm(mz[PARTS == 2 ? 2 : 0][i >> 1], mz[PARTS == 2 ? 3 : 0][i >> 1], half) & 0x000f000fu;
 #pragma unroll
                     for (int k = 0; k < 8; ++k) c[k] = q4_less(c[k], (k & 2 ? y1 : y0) << (k & 1 ? 4 : 0));
+                }
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     const float p0 = y[n][0] * s0, p1 = y[n][1] * s0, p2 = y[n][2] * s1, p3 = y[n][3] * s1;
@@ -432,7 +445,11 @@ attend_kernel(const Args a) {
                     }
                     mma_f16(O[n][i][0], c[0], c[1], c[2], c[3], b0, b1);
                     mma_f16(O[n][i][1], c[4], c[5], c[6], c[7], b0, b1);
-                    mma_f16(Z[PARTS == 1 ? n : 0][i], y0, y0, y1, y1, b0, b1);        // Σ p s z with the same rounded numbers, in every row
+                    // (the zeros are taken off with the same rounded numbers, so that a value of zero adds exactly nothing)
+                    const float z0 = zero_at(m0[j], i), z1 = zero_at(m1[j], i);
+                    const float2 f0 = __half22float2(*(const __half2*)&h0), f1 = __half22float2(*(const __half2*)&h1);
+                    zs[n][i][0] = fmaf(f0.x, z0, fmaf(f1.x, z1, zs[n][i][0]));
+                    zs[n][i][1] = fmaf(f0.y, z0, fmaf(f1.y, z1, zs[n][i][1]));
                 }
             }
         }
@@ -443,7 +460,8 @@ attend_kernel(const Args a) {
                 if (it + j < n_pages) mbar_arrive(smem_u32(&empty[(it + j) % STAGES]));
     }
 
-    // each warp's sums over its lanes; then the warps', in their order, in shared memory (where the pages were)
+    // each warp's sums over its lanes, its columns' numbers in shared memory (where the pages were); then the warps', in their order
+    __syncthreads();
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -451,6 +469,9 @@ attend_kernel(const Args a) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 sum[n][e] += __shfl_xor_sync(0xffffffffu, sum[n][e], o);
+                if (PARTS == 1)
+#pragma unroll
+                    for (int i = 0; i < NG; ++i) zs[n][i][e] += __shfl_xor_sync(0xffffffffu, zs[n][i][e], o);
             }
             poison[n] |= __shfl_xor_sync(0xffffffffu, poison[n], o);
         }
@@ -460,62 +481,54 @@ attend_kernel(const Args a) {
                 ref_s[warp][n * 8 + 2 * t + e] = top[n][e] == -INFINITY && sum[n][e] == 0.0f ? -INFINITY : ref[n][e];
                 sum_s[warp][n * 8 + 2 * t + e] = sum[n][e];
             }
-    }
-    __syncthreads();
-    float* acc = (float*)smem;                                       // [column][HD]
-    for (int w = 0; w < WARPS; ++w) {
-        if (warp == w) {
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+        for (int i = 0; i < NG; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const int c = n * 8 + 2 * t + e;
-                    float big = ref_s[0][c];
-#pragma unroll
-                    for (int k = 1; k < WARPS; ++k) big = fmaxf(big, ref_s[k][c]);
-                    const float f = ref_s[w][c] == -INFINITY ? 0.0f : ex2(ref_s[w][c] - big);
-#pragma unroll
-                    for (int i = 0; i < NG; ++i)
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            float2* to = (float2*)(acc + c * HD + 32 * i + 4 * g + 2 * h);
-                            const float z = PARTS == 1 ? Z[PARTS == 1 ? n : 0][i][e] : 0.0f, up = PARTS == 1 ? 16777216.0f : 1.0f;
-                            float2 v = make_float2((O[n][i][h][e] - z) * up * f, (O[n][i][h][2 + e] * 0.0625f - z) * up * f);
-                            if (f == 0.0f) v = make_float2(0.0f, 0.0f);
-                            if (poison[n] >> (2 * i + e) & 1) v.x = v.y = __int_as_float(0x7fc00000);
-                            if (w > 0) { v.x += to->x; v.y += to->y; }
-                            *to = v;
-                        }
+                    float2 v = make_float2(fmaf(O[n][i][h][e], PARTS == 2 ? 1.0f : 16777216.0f, -zs[n][i][e]), fmaf(O[n][i][h][2 + e], PARTS == 2 ? 0.0625f : 1048576.0f, -zs[n][i][e]));
+                    if (poison[n] >> (2 * i + e) & 1) v.x = v.y = __int_as_float(0x7fc00000);
+                    *(float2*)(acc + (warp * COLS + n * 8 + 2 * t + e) * ROW + 32 * i + 4 * g + 2 * h) = v;
                 }
-        }
-        __syncthreads();
     }
+    __syncthreads();
     if (failed) return;
     for (int c = warp; c < n_cols; c += WARPS) {
-        float big = ref_s[0][c], total = 0.0f;
+        float big = ref_s[0][c], total = 0.0f, f[WARPS];
 #pragma unroll
         for (int k = 1; k < WARPS; ++k) big = fmaxf(big, ref_s[k][c]);
 #pragma unroll
-        for (int k = 0; k < WARPS; ++k) total += ref_s[k][c] == -INFINITY ? 0.0f : sum_s[k][c] * ex2(ref_s[k][c] - big);
-        const int tok = tok0 + (col0 + c) / G, head = kvh * G + (col0 + c) % G;
-        const size_t out_row = (size_t)tok * a.nh + head;
+        for (int k = 0; k < WARPS; ++k) {
+            f[k] = ref_s[k][c] == -INFINITY ? 0.0f : ex2(ref_s[k][c] - big);
+            total += ref_s[k][c] == -INFINITY ? 0.0f : sum_s[k][c] * f[k];
+        }
+        float v[NG];
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+            v[i] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < WARPS; ++k)
+                if (ref_s[k][c] != -INFINITY) v[i] = fmaf(f[k], acc[(k * COLS + c) * ROW + 32 * i + lane], v[i]);
+        }
+        const int head = kvh * G + (col0 + c) % G;
+        const size_t out_row = (size_t)(tok0 + (col0 + c) / G) * a.nh + head;
         if (a.n_chunks > 1) {
             float* part = a.part + (out_row * a.n_chunks + chunk) * HD;
-            for (int d = lane; d < HD; d += 32) part[d] = acc[c * HD + d];
+#pragma unroll
+            for (int i = 0; i < NG; ++i) part[32 * i + lane] = v[i];
             if (lane == 0) ((float2*)(a.part + (size_t)a.T * a.nh * a.n_chunks * HD))[out_row * a.n_chunks + chunk] = make_float2(big, total);
             continue;
         }
-        float f = 1.0f;
+        float down = 1.0f;
         if (a.sink) {
             const float y = a.sink[head] * LOG2E, most = fmaxf(big, y);
-            f = big == -INFINITY ? 0.0f : ex2(big - most);
-            total = total * f + ex2(y - most);
+            down = big == -INFINITY ? 0.0f : ex2(big - most);
+            total = total * down + ex2(y - most);
         }
-        const float inv = big == -INFINITY ? 0.0f : f / total;       // (no key seen: zeros)
-        for (int d = lane; d < HD; d += 32) {
-            const float v = big == -INFINITY ? 0.0f : acc[c * HD + d] * inv;
-            sp_st((TQ*)a.out, out_row * HD + d, v);
-        }
+#pragma unroll
+        for (int i = 0; i < NG; ++i)                                 // (no key seen: zeros)
+            sp_st((TQ*)a.out, out_row * HD + 32 * i + lane, big == -INFINITY ? 0.0f : v[i] * down / total);
     }
 }
 
@@ -562,9 +575,8 @@ join_kernel(const Args a, int hd) {
 
 template <typename TQ, int NG, int NT>
 int launch(const Args& a, int n_seqs, int tiles, cudaStream_t stream) {
-    constexpr int PARTS = sizeof(TQ) == 4 ? 2 : 1, RING = STAGES * kv4_tile_bytes(32 * NG), ACC = 8 * NT * 32 * NG * 4;
-    constexpr int SMEM = (RING > ACC ? RING : ACC) + (NT == 1 && PARTS == 1 ? 0 : NT * NG * PARTS * 512);
-    static_assert(RING >= ACC, "the joined sums lie where the pages were");
+    constexpr int HD = 32 * NG, PARTS = sizeof(TQ) == 4 ? 2 : 1, RING = STAGES * kv4_tile_bytes(HD), SUMS = WARPS * 8 * NT * (HD + 8) * 4;
+    constexpr int HELD = RING + (NT == 1 && PARTS == 1 ? 0 : NT * NG * PARTS * 512), SMEM = HELD > SUMS ? HELD : SUMS;
     static SpPerDevice configured;
     if (!configured.done()) {
         cudaError_t e = cudaFuncSetAttribute(attend_kernel<TQ, NG, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
@@ -582,7 +594,6 @@ template <typename TQ, int NG>
 int launch(const Args& a, int n_seqs, int nt, int max_new, cudaStream_t stream) {
     const int G = a.nh / a.nkv, tiles = (max_new * G + 8 * nt - 1) / (8 * nt);
     if ((long long)a.nkv * tiles > 65535 || n_seqs > 65535) SP_FAIL("kv4_attention: %d sequences of %d tokens, %d kv heads", n_seqs, max_new, a.nkv);
-    if (nt == 4) return launch<TQ, NG, 4>(a, n_seqs, tiles, stream);
     if (nt == 2) return launch<TQ, NG, 2>(a, n_seqs, tiles, stream);
     return launch<TQ, NG, 1>(a, n_seqs, tiles, stream);
 }
@@ -603,7 +614,7 @@ int launch(const Args& a, int n_seqs, int nt, int max_new, int hd, cudaStream_t 
 SP_API long long sp_kv4_attend_scratch(int T, int nh, int hd, int n_chunks) { return n_chunks > 1 ? (long long)T * nh * n_chunks * (hd + 2) : 0; }
 
 // out [T, nh·hd] for queries q of the same shape and type (bfloat16 or float32). ``seq_start`` [n_seqs + 1], null: one token a
-// sequence. ``max_new``: the most tokens of a sequence. ``nt``: 8 nt columns a CTA (1, 2 or 4). ``chunk_pages``, ``n_chunks``:
+// sequence. ``max_new``: the most tokens of a sequence. ``nt``: 8 nt columns a CTA (1 or 2). ``chunk_pages``, ``n_chunks``:
 // the split of the keys, from the first that a CTA's tokens see.
 SP_API int sp_kv4_attend(const void* q, void* out, int dt, const void* pool, const int* seq_start, const int* positions, const int* seq_row,
                          const int* page_table, int max_pages, int page_size, int T, int n_seqs, int max_new, int nh, int nkv, int hd,
@@ -613,7 +624,7 @@ SP_API int sp_kv4_attend(const void* q, void* out, int dt, const void* pool, con
     if (hd <= 0 || hd % 32 || hd > KV4_MAX_HD) SP_FAIL("kv4_attention: head sizes 32, 64, 96 and 128, got %d", hd);
     if (page_size != KV4_PAGE) SP_FAIL("kv4_attention: pages of %d positions, got %d", KV4_PAGE, page_size);
     if (nkv <= 0 || nh <= 0 || nh % nkv) SP_FAIL("kv4_attention: %d heads are no multiple of %d kv heads", nh, nkv);
-    if (nt != 1 && nt != 2 && nt != 4) SP_FAIL("kv4_attention: 8, 16 or 32 columns a CTA, got 8 x %d", nt);
+    if (nt != 1 && nt != 2) SP_FAIL("kv4_attention: 8 or 16 columns a CTA, got 8 x %d", nt);
     if (window < 0 || max_new <= 0 || (!seq_start && (max_new != 1 || T != n_seqs))) SP_FAIL("kv4_attention: window %d, %d tokens of %d sequences, at most %d of one", window, T, n_seqs, max_new);
     if (chunk_pages <= 0 || n_chunks <= 0 || n_chunks > 65535) SP_FAIL("kv4_attention: %d chunks of %d pages", n_chunks, chunk_pages);
     if (!(scale > 0.0f) || scale > 1e30f) SP_FAIL("kv4_attention: a positive scale is wanted, got %g", scale);

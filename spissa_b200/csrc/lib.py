@@ -1945,7 +1945,7 @@ def kv4_unpack_pages(pool, meta, k_out, v_out, table, step, window, nkv, hd) -> 
 def kv4_attend_plan(n_seqs: int, nkv: int, cols: int, pages: int) -> tuple:
     """(tiles of eight columns a CTA takes, pages per chunk, chunks) for ``kv4_attend``: ``cols`` query columns (heads of a kv head
     times tokens) of the sequence with the most, ``pages`` of keys that the longest sequence's tokens see."""
-    nt = 1 if cols <= 8 else 2 if cols <= 16 else 4
+    nt = 1 if cols <= 8 else 2
     base = n_seqs * nkv * -(-cols // (8 * nt))
     n_chunks = min(max(1, -(-pages // 2)), max(1, round((592 if nt == 1 else 296) / base)))
     chunk_pages = -(-pages // n_chunks)
