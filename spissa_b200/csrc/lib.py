@@ -1942,14 +1942,25 @@ def kv4_unpack_pages(pool, meta, k_out, v_out, table, step, window, nkv, hd) -> 
         c_void_p(_stream())))
 
 
+@functools.lru_cache(maxsize=4096)
 def kv4_attend_plan(n_seqs: int, nkv: int, cols: int, pages: int) -> tuple:
     """(tiles of eight columns a CTA takes, pages per chunk, chunks) for ``kv4_attend``: ``cols`` query columns (heads of a kv head
-    times tokens) of the sequence with the most, ``pages`` of keys that the longest sequence's tokens see."""
+    times tokens) of the sequence with the most, ``pages`` of keys that the longest sequence's tokens see.
+
+    By rounds of the CTAs that find room (four of an SM with eight columns, two with sixteen) times what one takes: its pages and about three
+    more for setting up and joining its warps' sums; the chunks' joining costs two and a third of one per chunk. Measured (us, as
+    chosen / otherwise): 64 sequences of 2,048 keys 50 in one chunk, 52 in two, 56 in four; 3 of about 50,000 71 in 24, 77 in 16, 81 in
+    32; one of 2,048 10.7 in eleven, 10.3 in seven, 12.3 in seventeen; 40 tokens behind 6,000 46 in three, 52 in six."""
     nt = 1 if cols <= 8 else 2
-    base = n_seqs * nkv * -(-cols // (8 * nt))
-    n_chunks = min(max(1, -(-pages // 2)), max(1, round((592 if nt == 1 else 296) / base)))
-    chunk_pages = -(-pages // n_chunks)
-    return nt, chunk_pages, -(-pages // chunk_pages)
+    base, room = n_seqs * nkv * -(-cols // (8 * nt)), 592 if nt == 1 else 296
+    best = None
+    for n in range(1, min(pages, max(1, 2 * room // base)) + 1):
+        each = -(-pages // n)
+        n = -(-pages // each)
+        cost = -(-base * n // room) * (each + 3) + (2 + 0.35 * n if n > 1 else 0)
+        if best is None or cost < best[0]:
+            best = cost, each, n
+    return nt, best[1], best[2]
 
 
 def kv4_attend(q, pool, out, meta, seq_start, n_seqs: int, max_new: int, longest: int, nh, nkv, hd, window, scale, sink=None, plan=None) -> None:
