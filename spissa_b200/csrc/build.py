@@ -64,12 +64,14 @@ MODULES = {
     "rglru": "rglru_kernels.cu",
     "mlstm": "mlstm_kernels.cu",
     "q4": "q4_kernels.cu",
+    "q4_tc": "q4_tc.cu",
     "kv4": "kv4_kernels.cu",
     "kv4_attention": "kv4_attention.cu",
 }
 # headers that only these modules include
 OWN_HEADERS = {
-    "q4_kernels.cu": ["q4.cuh"],
+    "q4_kernels.cu": ["q4.cuh", "q4w.cuh"],
+    "q4_tc.cu": ["q4.cuh", "q4w.cuh"],
     "kv4_kernels.cu": ["q4.cuh", "kv4.cuh"],
     "kv4_attention.cu": ["q4.cuh", "kv4.cuh"],
 }

@@ -47,6 +47,10 @@ def load(module: str) -> ctypes.CDLL:
             # declared once: plain integers pass, without an object made for each of a call's arguments
             lib.sp_q4_gemv.argtypes = [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_longlong,
                                        c_longlong, c_int, c_int, c_float, c_void_p]
+        if module == "q4_tc":
+            lib.sp_q4_tc_estimate.restype = ctypes.c_double
+            lib.sp_q4_tc.argtypes = [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_longlong, c_longlong,
+                                     c_int, c_int, c_float, c_void_p, c_void_p]
         if module == "kv4":
             lib.sp_kv4_store.argtypes = [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p] + \
                 [c_int] * 6 + [c_void_p]
@@ -1831,7 +1835,8 @@ def q4_unpack(codes, scales, out, group: int, half: int = 0, block: int = 0) -> 
         c_void_p(_stream())))
 
 
-Q4_GEMV_ROWS = 16         # rows of x that ``q4_gemv`` takes
+Q4_GEMV_ROWS = 16         # rows of x that ``q4_gemv`` takes,
+Q4_TC_ROWS = 1024         # and ``q4_tc``
 
 
 def q4_gemv(x, codes, scales, out, rows: int, group: int, half: int = 0, mode=TC_STORE, act=ACT_SILU, mult: float = 1.0) -> None:
@@ -1843,6 +1848,22 @@ def q4_gemv(x, codes, scales, out, rows: int, group: int, half: int = 0, mode=TC
                         x.stride(0), out.stride(0), mode, act, mult, _stream())
     if rc:
         _check("q4", rc)
+
+
+@functools.lru_cache(maxsize=None)
+def q4_tc_estimate(M: int, rows: int, K: int, group: int, half: int = 0) -> float:
+    """The time that ``q4_tc`` is expected to take, ns."""
+    return load("q4_tc").sp_q4_tc_estimate(M, rows, K, group, half)
+
+
+def q4_tc(x, codes, scales, out, rows: int, group: int, half: int = 0, mode=TC_STORE, act=ACT_SILU, mult: float = 1.0) -> None:
+    """``q4_gemv`` for up to 1,024 bfloat16 rows of x, on the tcgen05 tensor cores."""
+    lib = load("q4_tc")
+    M, K = x.shape
+    rc = lib.sp_q4_tc(x.data_ptr(), codes.data_ptr(), scales.data_ptr(), out.data_ptr(), dt_code(out), M, rows, K, group, half, x.stride(0),
+                      out.stride(0), mode, act, mult, status_word(x.device).data_ptr(), _stream())
+    if rc:
+        _check("q4_tc", rc)
 
 
 # ------------------------------------------------------------------ four bits: keys and values

@@ -1,12 +1,6 @@
 // Weights of four bits (q4.cuh): packing, unpacking, and the product for up to 16 tokens.
 //
-// Layout. Rows of W come in tiles of 16, columns in blocks of 128, both filled up with zeros. A block of a tile is 1,024 bytes, two
-// pieces of 64 columns: lane 4 g + t of a warp owns 16 bytes of each, the words (row g: columns 8 t.., 32 + 8 t..), (row g + 8:
-// the same), that is, the A operand of four m16n8k16 products in one load. Scales and zeros: [tile][block][row g][group of the
-// block][row g, row g + 8], 16 bits each. A gated product's rows alternate by tiles: 16 gate rows, the 16 up rows of the same
-// outputs.
-#include "q4.cuh"
-#include <cuda_fp16.h>
+#include "q4w.cuh"
 
 SP_API const char* sp_q4_last_error() { return sp_error_text; }
 SP_DEFINE_RANGE_API(q4)
@@ -21,16 +15,6 @@ __device__ __forceinline__ int source_row(int packed, int rows, const RowMap& m)
     const int o = (packed >> 5) * 16 + (packed & 15), up = (packed >> 4) & 1;
     if (o >= m.half) return -1;
     return m.block ? (o / m.block) * 2 * m.block + up * m.block + o % m.block : up * m.half + o;
-}
-
-constexpr int BLOCK = 128;         // columns
-
-__device__ __forceinline__ size_t word_at(int row, int k8, int blocks) {             // the word of columns 8 k8 .. of a packed row
-    return ((((size_t)(row >> 4) * blocks + (k8 >> 4)) * 2 + ((k8 >> 3) & 1)) * 32 + (row & 7) * 4 + (k8 & 3)) * 4 + ((row >> 3) & 1) * 2 + ((k8 >> 2) & 1);
-}
-__device__ __forceinline__ size_t meta_at(int row, int k8, int blocks, int group) {
-    const int per = BLOCK / group;
-    return ((((size_t)(row >> 4) * blocks + (k8 >> 4)) * 8 + (row & 7)) * per + (8 * k8 % BLOCK) / group) * 2 + ((row >> 3) & 1);
 }
 
 // A thread packs eight columns of a row; 4, 8 or 16 neighbouring threads share a group.
@@ -59,8 +43,8 @@ __global__ void pack_kernel(const void* w, int dt, long long ldw, uint32_t* code
 #pragma unroll
     for (int i = 0; i < 8; ++i) word |= (uint32_t)q4_code(x[i], g) << (4 * (i / 2 + 4 * (i & 1)));
     if (!kept) return;
-    codes[word_at(row, k8, blocks)] = word;
-    if ((8 * k8) % group == 0) meta[meta_at(row, k8, blocks, group)] = (uint16_t)q4_meta(g);
+    codes[q4w_word_at(row, k8, blocks)] = word;
+    if ((8 * k8) % group == 0) meta[q4w_meta_at(row, k8, blocks, group)] = (uint16_t)q4_meta(g);
 }
 
 // The numbers themselves, a warp a block of a tile at a time: its codes in two loads, eight neighbouring numbers in one store.
@@ -79,14 +63,14 @@ unpack_kernel(const uint4* codes, const uint16_t* meta, T* out, int rows, int K,
     if (block >= blocks) return;
     const uint4* from = codes + ((size_t)tile * blocks + block) * 64 + lane;
     const uint4 w[2] = {from[0], from[32]};
-    const int per = BLOCK / group;
+    const int per = Q4W_BLOCK / group;
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
         const int dst = source_row(tile * 16 + g + 8 * r, rows, map);
         if (dst < 0) continue;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {                                // quarters of 32 columns
-            const int k = block * BLOCK + 32 * i + 8 * t;
+            const int k = block * Q4W_BLOCK + 32 * i + 8 * t;
             if (k >= K) break;
             const uint32_t m = meta[((((size_t)tile * blocks + block) * 8 + g) * per + 32 * i / group) * 2 + r];
             const uint32_t z = 0x43004300u | (m & 15u) * 0x10001u, s = (m & 0xfff0u) * 0x10001u;
@@ -190,7 +174,7 @@ constexpr int MOST_WARPS = 16;
 template <typename TX, int NT, int GROUP, int RT, int DEPTH>
 __global__ void __launch_bounds__(MOST_WARPS * 32)
 gemv_kernel(const TX* x, const Product p) {
-    constexpr int PARTS = sizeof(TX) == 4 ? 2 : 1, GROUPS = BLOCK / GROUP, META = 4 * GROUPS;        // META: bytes of a lane row's scales
+    constexpr int PARTS = sizeof(TX) == 4 ? 2 : 1, GROUPS = Q4W_BLOCK / GROUP, META = 4 * GROUPS;        // META: bytes of a lane row's scales
     extern __shared__ __align__(16) float4 red[];                    // [tile][share][column group][lane]
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, warps = p.sets * p.ki;
     const int rank = p.cs > 1 ? (int)cluster_rank() : 0, set = warp / p.ki, share = warp % p.ki;
@@ -225,11 +209,11 @@ gemv_kernel(const TX* x, const Product p) {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             const int token = n * 8 + g;
-            const TX* row = x + (size_t)min(token, p.M - 1) * p.ldx + (size_t)b * BLOCK + 8 * t;
+            const TX* row = x + (size_t)min(token, p.M - 1) * p.ldx + (size_t)b * Q4W_BLOCK + 8 * t;
             float v[4][8], top = 0.0f;
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                load8(row + 32 * q, there && token < p.M && b * BLOCK + 32 * q < p.K, v[q]);
+                load8(row + 32 * q, there && token < p.M && b * Q4W_BLOCK + 32 * q < p.K, v[q]);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[q][e]));                        // (NaN is left out)
             }
@@ -440,12 +424,11 @@ int check_sizes(const char* what, int rows, int K, int group, int half, int bloc
 }  // namespace
 
 // Rows of the packed weight (a multiple of 16): each half filled up for itself.
-SP_API int sp_q4_packed_rows(int rows, int half) { return half ? (half + 15) / 16 * 32 : (rows + 15) / 16 * 16; }
 
 SP_API int sp_q4_pack(const void* w, int dt, long long ldw, void* codes, void* meta, int rows, int K, int group, int half, cudaStream_t stream) {
     if (check_sizes("q4_pack", rows, K, group, half, 0)) return 1;
     if ((uintptr_t)codes & 15) SP_FAIL("q4_pack: the codes must start on a 16-byte boundary");
-    const int packed = sp_q4_packed_rows(rows, half), blocks = (K + BLOCK - 1) / BLOCK;
+    const int packed = q4w_tiles(rows, half) * 16, blocks = (K + Q4W_BLOCK - 1) / Q4W_BLOCK;
     pack_kernel<<<dim3(packed, (blocks * 16 + 127) / 128), blocks < 8 ? (blocks * 16 + 31) / 32 * 32 : 128, 0, stream>>>(w, dt, ldw, (uint32_t*)codes, (uint16_t*)meta, rows, K,
                                                                              blocks, group, RowMap{half, 0});
     SP_CHECK_LAUNCH("q4_pack");
@@ -456,7 +439,7 @@ SP_API int sp_q4_pack(const void* w, int dt, long long ldw, void* codes, void* m
 SP_API int sp_q4_unpack(const void* codes, const void* meta, void* out, int dt, int rows, int K, int group, int half, int block, cudaStream_t stream) {
     if (check_sizes("q4_unpack", rows, K, group, half, block)) return 1;
     if ((uintptr_t)out & 15) SP_FAIL("q4_unpack: the output must start on a 16-byte boundary");
-    const int packed = sp_q4_packed_rows(rows, half), blocks = (K + BLOCK - 1) / BLOCK;
+    const int packed = q4w_tiles(rows, half) * 16, blocks = (K + Q4W_BLOCK - 1) / Q4W_BLOCK;
     const dim3 grid(packed / 16, (blocks + 7) / 8), block_dim(blocks < 8 ? blocks * 32 : 256);
     const RowMap map{half, block};
     if (dt == SP_DT_F32) unpack_kernel<<<grid, block_dim, 0, stream>>>((const uint4*)codes, (const uint16_t*)meta, (float*)out, rows, K, blocks, group, map);
@@ -476,7 +459,7 @@ SP_API int sp_q4_gemv(const void* x, int x_dt, const void* codes, const void* me
     if (mode == MODE_ACCUMULATE && out_dt != SP_DT_F32) SP_FAIL("q4_gemv: accumulation needs a float32 output");
     if (((uintptr_t)x & 15) || (ldx * (x_dt == SP_DT_F32 ? 4 : 2)) % 16) SP_FAIL("q4_gemv: rows of x must start on 16-byte boundaries");
     if (((uintptr_t)codes & 15) || ((uintptr_t)meta & 15)) SP_FAIL("q4_gemv: codes and scales must start on 16-byte boundaries");
-    const int packed = sp_q4_packed_rows(rows, half), blocks = (K + BLOCK - 1) / BLOCK;
+    const int packed = q4w_tiles(rows, half) * 16, blocks = (K + Q4W_BLOCK - 1) / Q4W_BLOCK;
     const Product p{(const uint8_t*)codes, (const uint8_t*)meta, out, ldx, ldo, out_dt, M, rows, packed / 16, blocks, K, mode, half, 1, 1, 1, 1, SpGate{act, mult}};
     return x_dt == SP_DT_F32 ? launch_gemv<float>(x, p, group, stream) : launch_gemv<__nv_bfloat16>(x, p, group, stream);
 }

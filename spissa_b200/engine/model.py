@@ -83,7 +83,7 @@ class Model:
         for p in self.parts():
             walk(p)
         if rt is not None and rt.weight_bits == 4:
-            own.append("q4")
+            own += ["q4"] + ["q4_tc"] * (act_dtype == torch.bfloat16)
         if rt is not None and rt.cache_bits == 4:
             own += ["kv4", "kv4_attention"]
         if act_dtype != torch.bfloat16:

@@ -155,7 +155,8 @@ class GatedLinear:
 
 class Linear4:
     """y = x · Ŵᵀ, Ŵ the numbers that ``weight`` [out, in] becomes in four bits, in groups of ``group`` (32, 64 or 128) columns;
-    in a multiple of the group. Called as ``Linear``: x bfloat16 or float32."""
+    in a multiple of the group. Called as ``Linear``: x bfloat16 or float32. Up to 16 rows stream the codes, some dozens of bfloat16
+    rows multiply with them on the tcgen05 cores, more (and float32 ones) unpack the weight first."""
 
     def __init__(self, weight: torch.Tensor, group: int = 64):
         if weight.dim() != 2:
@@ -186,10 +187,12 @@ class Linear4:
                 raise ValueError("accumulation needs the tensor to add into")
             out = x.new_empty((x.shape[0], self.out_features), dtype=out_dtype)
         M = check4(self, x, out, self.out_features, accumulate)
-        if 0 < M <= K.Q4_GEMV_ROWS:
-            K.q4_gemv(on_boundaries(x), self.codes, self.scales, out, self.out_features, self.group, 0, K.TC_ACCUMULATE if accumulate else K.TC_STORE)
-        elif M:
-            Linear(self.unpacked(x.dtype))(x, out=out, accumulate=accumulate)
+        if M == 0:
+            return out
+        way, mode = product4(self, x, self.out_features), K.TC_ACCUMULATE if accumulate else K.TC_STORE
+        if way == "unpack":
+            return Linear(self.unpacked(x.dtype))(x, out=out, accumulate=accumulate)
+        (K.q4_gemv if way == "gemv" else K.q4_tc)(on_boundaries(x), self.codes, self.scales, out, self.out_features, self.group, 0, mode)
         return out
 
 
@@ -219,11 +222,31 @@ class GatedLinear4:
     def __call__(self, x: torch.Tensor, act_dtype) -> torch.Tensor:
         out = x.new_empty((x.shape[0], self.intermediate), dtype=act_dtype)
         M = check4(self, x, out, self.intermediate, False)
-        if 0 < M <= K.Q4_GEMV_ROWS:
-            K.q4_gemv(on_boundaries(x), self.codes, self.scales, out, 2 * self.intermediate, self.group, self.intermediate, K.TC_SILU_MUL, self.act, self.mult)
-        elif M:
+        if M == 0:
+            return out
+        way = product4(self, x, 2 * self.intermediate, self.intermediate)
+        if way == "unpack":
             return self.unpacked(x.dtype)(x, act_dtype)
+        (K.q4_gemv if way == "gemv" else K.q4_tc)(on_boundaries(x), self.codes, self.scales, out, 2 * self.intermediate, self.group,
+                                                  self.intermediate, K.TC_SILU_MUL, self.act, self.mult)
         return out
+
+
+def product4(lin, x, rows: int, half: int = 0) -> str:
+    """The way of a product of four-bit weights (``rows`` of them): "gemv" streams the codes (q4_kernels.cu), "tc" multiplies with
+    them on the tcgen05 cores (q4_tc.cu), "unpack" takes the weight apart in memory. Measured, us:
+      9 to 16 rows of x, weight 14336 x 4096 gate and up: gemv 51, tc 32; 4096 x 4096: 11, 9.6; 2048 x 2048: 6.4, 7.7;
+      256 rows, gate and up: tc 73, unpack 111; 4096 x 4096: 17, 25 (more sizes: q4_tc.cu).
+    Beyond 256 rows tc takes each code apart more than once, unpack writes and reads 2 bytes a number once: an estimate of each
+    decides, unpack's as 2,300 numbers a nanosecond and a product of 1.5 PFLOP/s that starts in 9 us."""
+    M, numbers = x.shape[0], rows * lin.in_features
+    if M <= 8 or (M <= K.Q4_GEMV_ROWS and (numbers < 1 << 23 or x.dtype != torch.bfloat16)):
+        return "gemv"
+    if x.dtype != torch.bfloat16 or M > K.Q4_TC_ROWS:
+        return "unpack"
+    if M <= 256 or K.q4_tc_estimate(M, rows, lin.in_features, lin.group, half) < numbers / 2300 + 9000 + M * numbers * 2 / 1.5e6:
+        return "tc"
+    return "unpack"
 
 
 def held_linear(weight: torch.Tensor, rt):
