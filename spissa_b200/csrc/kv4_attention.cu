@@ -45,7 +45,7 @@ struct Args {
     const float* sink;             // [nh] or null
     float* part;                   // [T * nh][n_chunks][hd], then [T * nh][n_chunks] (reference, sum); unused with one chunk
     int* status;
-    int max_pages, nh, nkv, window, chunk_pages, n_chunks, T;
+    int max_pages, nh, nkv, window, chunk_pages, n_chunks, T, n_seqs;
     float scale;
     SpRange rg;
 };
@@ -539,7 +539,7 @@ join_kernel(const Args a, int hd) {
     sp_wait_for_predecessor();
     const int lane = threadIdx.x & 31;
     const size_t rows = (size_t)a.T * a.nh, row = (size_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (row >= rows) return;
+    if (row >= rows || (a.seq_start && row >= (size_t)a.seq_start[a.n_seqs] * a.nh)) return;        // rows behind the last sequence stay as they are
     const float* part = a.part + row * a.n_chunks * hd;
     const float2* heads = (const float2*)(a.part + rows * a.n_chunks * hd) + row * a.n_chunks;
     float big = -INFINITY;
@@ -631,6 +631,6 @@ SP_API int sp_kv4_attend(const void* q, void* out, int dt, const void* pool, con
     if (((uintptr_t)q & 15) || ((uintptr_t)pool & 15)) SP_FAIL("kv4_attention: queries and pages must start on 16-byte boundaries");
     if (sp_kv4_attend_scratch(T, nh, hd, n_chunks) > scratch_floats) SP_FAIL("kv4_attention: %lld floats of scratch are needed, got %lld", sp_kv4_attend_scratch(T, nh, hd, n_chunks), scratch_floats);
     const Args a{q, out, (const uint8_t*)pool, seq_start, positions, seq_row, page_table, sink, scratch, status,
-                 max_pages, nh, nkv, window, chunk_pages, n_chunks, T, scale, sp_range_host};
+                 max_pages, nh, nkv, window, chunk_pages, n_chunks, T, n_seqs, scale, sp_range_host};
     return dt == SP_DT_F32 ? launch<float>(a, n_seqs, nt, max_new, hd, stream) : launch<__nv_bfloat16>(a, n_seqs, nt, max_new, hd, stream);
 }

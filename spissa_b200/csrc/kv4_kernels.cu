@@ -188,8 +188,8 @@ unpack_pages_kernel(const uint8_t* pool, T* k_out, T* v_out, int* table, const i
     if (mine) atomicAdd(&before, mine);
     __syncthreads();
     const int out = before + entry, row = sp_checked_row(seq_row[b], rg);
-    if (out >= n_out) return;                                        // (the host counted fewer pages than the lengths say)
-    if (head == 0 && threadIdx.x == 0) table[(size_t)b * max_pages + entry] = out;
+    if (head == 0 && threadIdx.x == 0) table[(size_t)b * max_pages + entry] = out < n_out ? out : 0;
+    if (out >= n_out || seq_start[b + 1] == seq_start[b]) return;    // (the host counted fewer pages than the lengths say; no queries)
     if (window && (entry + 1) * KV4_PAGE <= positions[seq_start[b]] + 1 - window) return;      // the first query's
     const int page = sp_checked_page(page_table[(size_t)row * max_pages + entry], rg);
     const uint8_t* tile = pool + ((size_t)page * nkv + head) * kv4_tile_bytes(hd);

@@ -1953,6 +1953,9 @@ def kv4_unpack_pages(pool, meta, k_out, v_out, table, step, window, nkv, hd) -> 
     if table.dtype != torch.int32 or table.shape != pt.shape or k_out.shape != v_out.shape or k_out.dtype != v_out.dtype \
             or tuple(k_out.shape[1:]) != (nkv, 64, hd):
         raise KernelError(f"kv4_unpack_pages: two pools [pages, {nkv}, 64, {hd}] of one type and a table like the cache's are wanted")
+    if not (step.seq_len.dtype == step.seq_start.dtype == torch.int32) or step.seq_len.numel() < step.n_seqs or step.seq_start.numel() < step.n_seqs + 1 \
+            or meta.seq_slot.numel() < step.n_seqs or table.size(0) < step.n_seqs:
+        raise KernelError("kv4_unpack_pages: lengths, first tokens and table rows of every sequence are wanted, int32")
     _kv4_check("kv4_unpack_pages", pool, meta, 0, nkv, hd, k_out, v_out, table, step.seq_len, step.seq_start)
     lib = load("kv4")
     _declare_bounds("kv4", lib, _pool_pages(meta, pool), _table_rows(meta, pt), pool.device)
@@ -1994,6 +1997,10 @@ def kv4_attend(q, pool, out, meta, seq_start, n_seqs: int, max_new: int, longest
     if sink is not None and (sink.dtype != torch.float32 or sink.numel() != nh):
         raise KernelError("kv4_attend: the sinks are one float32 per query head")
     _kv4_check("kv4_attend", pool, meta, T, nkv, hd, q, out, seq_start, sink)
+    if T == 0 or n_seqs <= 0:
+        return
+    if max_new < 1 or longest < 1:
+        raise KernelError(f"kv4_attend: at most {max_new} tokens of a sequence, {longest} keys of the longest")
     if seq_start is not None and (seq_start.dtype != torch.int32 or seq_start.numel() < n_seqs + 1):
         raise KernelError("kv4_attend: the sequences' first tokens are int32, one more than sequences")
     lib = load("kv4_attention")

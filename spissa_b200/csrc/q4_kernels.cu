@@ -423,8 +423,6 @@ int check_sizes(const char* what, int rows, int K, int group, int half, int bloc
 
 }  // namespace
 
-// Rows of the packed weight (a multiple of 16): each half filled up for itself.
-
 SP_API int sp_q4_pack(const void* w, int dt, long long ldw, void* codes, void* meta, int rows, int K, int group, int half, cudaStream_t stream) {
     if (check_sizes("q4_pack", rows, K, group, half, 0)) return 1;
     if ((uintptr_t)codes & 15) SP_FAIL("q4_pack: the codes must start on a 16-byte boundary");

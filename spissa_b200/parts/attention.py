@@ -230,6 +230,8 @@ def attend_four_bits(q, step, cache, nh, nkv, hd, window, scale, sink=None):
     T = q.shape[0]
     if q.dtype not in (torch.bfloat16, torch.float32) or tuple(q.shape) != (T, nh * hd) or nh % nkv:
         raise K.KernelError(f"attention: queries are [tokens, {nh} x {hd}], bfloat16 or float32, of heads in equal groups")
+    if not scale > 0:
+        raise K.KernelError(f"attention over a four-bit cache takes a positive scale, got {scale}")
     if step.all_single or step.max_new * (nh // nkv) <= SPLIT4_COLUMNS:
         out = torch.empty_like(q)
         # (a decode step by its length's bucket, as below: run directly and replayed from a graph it adds up in the same order)

@@ -281,5 +281,6 @@ def check4(lin, x, out, out_features: int, accumulate: bool) -> int:
 
 
 def on_boundaries(x):
-    """``x``, or a copy of it where its rows do not start on 16-byte boundaries (columns of wider rows, an odd offset)."""
-    return x if (x.data_ptr() | x.stride(0) * x.element_size()) % 16 == 0 else x.clone(memory_format=torch.contiguous_format)
+    """``x``, or a copy of it where its rows do not start on 16-byte boundaries (columns of wider rows, an odd offset) or overlap (one row
+    for all)."""
+    return x if (x.data_ptr() | x.stride(0) * x.element_size()) % 16 == 0 and x.stride(0) >= x.shape[1] else x.clone(memory_format=torch.contiguous_format)
