@@ -48,7 +48,7 @@ __global__ void __launch_bounds__(256)
 store_kernel(const float* qkv, TQ* q_out, uint8_t* pool, Place place, const float* inv_freq, int T, int per_block, int nh, int nkv, int rd, int write_kv) {
     constexpr int HD = 32 * NG, PER_HEAD = HD / 4, TILE = kv4_tile_bytes(HD);
     __shared__ double2 turns[STORE_TOKENS][HD / 2];                  // cos, sin
-    __shared__ float2 turns32[STORE_TOKENS][HD / 2];                 // the same rounded, for q
+    __shared__ __align__(16) float cos32[STORE_TOKENS][HD / 2], sin32[STORE_TOKENS][HD / 2];      // the same rounded, for q
     __shared__ int places[STORE_TOKENS][2];                          // page (or -1), place in it
     const int t0 = blockIdx.x * per_block, n_t = min(per_block, T - t0), half = rd >> 1;
     for (int i = threadIdx.x; i < n_t * half; i += blockDim.x) {
@@ -56,7 +56,8 @@ store_kernel(const float* qkv, TQ* q_out, uint8_t* pool, Place place, const floa
         double s, c;
         sincos((double)place.positions[t0 + k] * (double)inv_freq[j], &s, &c);
         turns[k][j] = make_double2(c, s);
-        turns32[k][j] = make_float2((float)c, (float)s);
+        cos32[k][j] = (float)c;
+        sin32[k][j] = (float)s;
     }
     if (threadIdx.x < n_t) {
         const int pos = place.positions[t0 + threadIdx.x];
@@ -94,11 +95,11 @@ store_kernel(const float* qkv, TQ* q_out, uint8_t* pool, Place place, const floa
                     float* a = &v.x;
                     const float* b = &os[i].x;
                     if (is_q) {
+                        const float4 c4 = *(const float4*)&cos32[k][at], s4 = *(const float4*)&sin32[k][at];
+                        const float* c = &c4.x;
+                        const float* s = &s4.x;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float2 w = turns32[k][at + e];
-                            a[e] = w.x * a[e] + (first ? -w.y : w.y) * b[e];
-                        }
+                        for (int e = 0; e < 4; ++e) a[e] = c[e] * a[e] + (first ? -s[e] : s[e]) * b[e];
                     } else {
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
