@@ -220,10 +220,17 @@ q4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ 
                 if (c0 + j < count) asm volatile("st.shared.b32 [%0], %1;" ::"r"(to + (uint32_t)(j * BW * 4)), "r"(r[j]) : "memory");
         }
     }
+    // The tensor memory goes back before the CTAs of a cluster wait for one another: a CTA that held it there could keep it from one of
+    // its own cluster on the same SM, or from a cluster of another stream that holds what this one's other CTAs wait for.
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(a.tmem_cols) : "memory");
+    }
     __syncwarp();
     // every CTA of the cluster has left its piece in its shared memory
     if (a.pieces > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-    else __syncthreads();
 
     if (warp >= 2 && !failed && !(a.status && *(volatile int*)a.status != 0)) {
         const bool gated = a.mode == MODE_SILU_MUL;
@@ -269,12 +276,6 @@ q4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ 
     __syncwarp();
     // nobody leaves (and frees its shared memory) before every CTA has read what it needs
     if (a.pieces > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-    tc_fence_before();
-    __syncthreads();
-    if (warp == 1) {
-        tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(a.tmem_cols) : "memory");
-    }
 }
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
