@@ -40,9 +40,11 @@ __device__ __forceinline__ void write_quad(__nv_bfloat16* to, float4 v) {
 
 constexpr int STORE_TOKENS = 4;             // of a block at most
 
-// A thread owns four neighbouring columns of a head; eight neighbouring threads a group. The angles are formed and their sine
-// and cosine taken in 64 bits, keys are rotated in 64 bits and rounded to 32 once: at position 100,000 an angle in 32 bits is
-// off by up to 0.004, and a key's code is a comparison that an error of the rotation may turn.
+// threads that a q head of so many units takes: 2^this
+__host__ __device__ __forceinline__ int store_shift(int units) { return units <= 4 ? 2 : units <= 8 ? 3 : units <= 16 ? 4 : 5; }
+
+// The angles are formed and their sine and cosine taken in 64 bits, keys are rotated in 64 bits and rounded to 32 once: at position
+// 100,000 an angle in 32 bits is off by up to 0.004, and a key's code is a comparison that an error of the rotation may turn.
 template <typename TQ, int NG>
 __global__ void __launch_bounds__(256)
 store_kernel(const float* qkv, TQ* q_out, uint8_t* pool, Place place, const float* inv_freq, int T, int per_block, int nh, int nkv, int rd, int write_kv) {
@@ -65,14 +67,44 @@ store_kernel(const float* qkv, TQ* q_out, uint8_t* pool, Place place, const floa
         places[threadIdx.x][1] = pos % KV4_PAGE;
     }
     __syncthreads();
-    const int quads = (nh + (write_kv ? 2 * nkv : 0)) * PER_HEAD;
+    // q: a thread turns four columns and their partners, or copies four that stay; a head takes 2^shift threads
+    const int pairs = rd >> 3, units = pairs + ((HD - rd) >> 2), shift = store_shift(units), stride = gridDim.y * blockDim.x;
+    for (int k = 0; k < n_t; ++k) {
+        const float* x = qkv + (size_t)(t0 + k) * (nh + 2 * nkv) * HD;
+        TQ* to = q_out + (size_t)(t0 + k) * nh * HD;
+        for (int u0 = blockIdx.y * blockDim.x + threadIdx.x; u0 < nh << shift; u0 += 2 * stride) {       // two units a turn, the second's columns on their way
+            float4 a[2], b[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int u = u0 + i * stride, un = u & ((1 << shift) - 1);
+                if (u >= nh << shift || un >= units) continue;
+                const float* from = x + (u >> shift) * HD + (un < pairs ? 4 * un : rd + 4 * (un - pairs));
+                a[i] = *(const float4*)from;
+                if (un < pairs) b[i] = *(const float4*)(from + half);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int u = u0 + i * stride, un = u & ((1 << shift) - 1);
+                if (u >= nh << shift || un >= units) continue;
+                TQ* at = to + (u >> shift) * HD + (un < pairs ? 4 * un : rd + 4 * (un - pairs));
+                if (un < pairs) {
+                    const float4 c = *(const float4*)&cos32[k][4 * un], s = *(const float4*)&sin32[k][4 * un];
+                    write_quad(at, make_float4(c.x * a[i].x - s.x * b[i].x, c.y * a[i].y - s.y * b[i].y, c.z * a[i].z - s.z * b[i].z, c.w * a[i].w - s.w * b[i].w));
+                    write_quad(at + half, make_float4(c.x * b[i].x + s.x * a[i].x, c.y * b[i].y + s.y * a[i].y, c.z * b[i].z + s.z * a[i].z, c.w * b[i].w + s.w * a[i].w));
+                } else {
+                    write_quad(at, a[i]);
+                }
+            }
+        }
+    }
+    if (!write_kv) return;
+    // keys and values: a thread four columns, eight neighbouring threads a group; from the other end of the token's blocks
+    const int quads = 2 * nkv * PER_HEAD;
     for (int k = 0; k < n_t; ++k) {
         const int page = places[k][0], slot = places[k][1];
-        const float* x = qkv + (size_t)(t0 + k) * (nh + 2 * nkv) * HD;
-        // Whole warps go through the loop together: eight lanes share a group (quads come in eights). Two quads a turn, so that the
-        // next one's columns are on their way.
-        const int stride = gridDim.y * blockDim.x;
-        for (int u0 = (blockIdx.y * blockDim.x + threadIdx.x) & ~31; u0 < quads; u0 += 2 * stride) {
+        const float* x = qkv + ((size_t)(t0 + k) * (nh + 2 * nkv) + nh) * HD;
+        // Whole warps go through the loop together: eight lanes share a group (quads come in eights).
+        for (int u0 = ((gridDim.y - 1 - blockIdx.y) * blockDim.x + threadIdx.x) & ~31; u0 < quads; u0 += 2 * stride) {
             float4 vs[2], os[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
@@ -80,36 +112,27 @@ store_kernel(const float* qkv, TQ* q_out, uint8_t* pool, Place place, const floa
                 vs[i] = os[i] = make_float4(0.f, 0.f, 0.f, 0.f);
                 if (u < quads) {
                     vs[i] = *(const float4*)(x + 4 * u);
-                    if (head < nh + nkv && d < rd) os[i] = *(const float4*)(x + 4 * u + (d < half ? half : -half));
+                    if (head < nkv && d < rd) os[i] = *(const float4*)(x + 4 * u + (d < half ? half : -half));
                 }
             }
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const int u = u0 + i * stride + (threadIdx.x & 31);
                 const bool in = u < quads;
+                if (!__any_sync(0xffffffffu, in)) break;
                 const int head = u / PER_HEAD, d = (u - head * PER_HEAD) * 4;
-                const bool is_q = head < nh, is_v = head >= nh + nkv, first = d < half;
+                const bool is_v = head >= nkv, first = d < half;
                 float4 v = vs[i];
                 if (in && !is_v && d < rd) {
                     const int at = first ? d : d - half;
                     float* a = &v.x;
                     const float* b = &os[i].x;
-                    if (is_q) {
-                        const float4 c4 = *(const float4*)&cos32[k][at], s4 = *(const float4*)&sin32[k][at];
-                        const float* c = &c4.x;
-                        const float* s = &s4.x;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) a[e] = c[e] * a[e] + (first ? -s[e] : s[e]) * b[e];
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const double2 w = turns[k][at + e];
-                            a[e] = (float)((double)a[e] * w.x + (double)b[e] * (first ? -w.y : w.y));
-                        }
+                    for (int e = 0; e < 4; ++e) {
+                        const double2 w = turns[k][at + e];
+                        a[e] = (float)((double)a[e] * w.x + (double)b[e] * (first ? -w.y : w.y));
                     }
                 }
-                if (in && is_q) write_quad(q_out + ((size_t)(t0 + k) * nh + head) * HD + d, v);
-                if (!__any_sync(0xffffffffu, in && !is_q)) continue;
                 float lo = fminf(fminf(fminf(v.x, v.y), fminf(v.z, v.w)), 0.0f), hi = fmaxf(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)), 0.0f);
                 const bool bad = q4_bad(v.x) || q4_bad(v.y) || q4_bad(v.z) || q4_bad(v.w);
 #pragma unroll
@@ -123,8 +146,8 @@ store_kernel(const float* qkv, TQ* q_out, uint8_t* pool, Place place, const floa
                 // a key's word holds eight columns: two threads'
                 uint32_t word = ((uint32_t)c0 | (uint32_t)c1 << 16 | (uint32_t)c2 << 4 | (uint32_t)c3 << 20) << (8 * (p8 & 1));
                 word |= __shfl_xor_sync(0xffffffffu, word, 1);
-                if (!in || is_q || page < 0) continue;
-                uint8_t* tile = pool + ((size_t)page * nkv + (is_v ? head - nh - nkv : head - nh)) * TILE;
+                if (!in || page < 0) continue;
+                uint8_t* tile = pool + ((size_t)page * nkv + (is_v ? head - nkv : head)) * TILE;
                 if (is_v) *(uint16_t*)(tile + kv4_v_codes(HD) + kv4_v_at(slot, p8, group, HD)) = (uint16_t)(c0 | c1 << 4 | c2 << 8 | c3 << 12);
                 else if (!(p8 & 1)) *(uint32_t*)(tile + kv4_k_at(slot, p8 >> 1, group, HD)) = word;
                 if (p8 == 0) *(uint16_t*)(tile + (is_v ? kv4_v_meta(HD) : kv4_k_meta(HD)) + ((is_v ? slot : kv4_key_slot(slot)) * NG + group) * 2) = (uint16_t)q4_meta(g);
@@ -225,9 +248,9 @@ SP_API int sp_kv4_store(const void* qkv, void* q_out, int q_dt, void* pool, cons
     if (write_kv && (!pool || !page_table || max_pages <= 0)) SP_FAIL("kv4_store: writing needs the pages and their table");
     if (((uintptr_t)qkv & 15) || ((uintptr_t)q_out & 15) || ((uintptr_t)pool & 15)) SP_FAIL("kv4_store: rows, q and pages must start on 16-byte boundaries");
     const Place place{token_seq, positions, seq_row, page_table, max_pages, sp_range_host};
-    const int quads = (nh + (write_kv ? 2 * nkv : 0)) * (hd / 4), sms = sp_sm_count() > 0 ? sp_sm_count() : 148;
+    const int units = (nh << store_shift(rd / 8 + (hd - rd) / 4)) + (write_kv ? 2 * nkv * (hd / 4) : 0), sms = sp_sm_count() > 0 ? sp_sm_count() : 148;
     // a few tokens: a token's heads over several blocks; many: several tokens to a block, whose angles are formed side by side
-    int per_block = T / (16 * sms), parts = (quads + 255) / 256;
+    int per_block = T / (16 * sms), parts = (units + 255) / 256;
     per_block = per_block < 1 ? 1 : per_block > STORE_TOKENS ? STORE_TOKENS : per_block;
     const int blocks = (T + per_block - 1) / per_block;
     if (blocks * parts > 6 * sms) parts = blocks >= 6 * sms ? 1 : (6 * sms + blocks - 1) / blocks;
