@@ -1967,16 +1967,17 @@ def kv4_unpack_pages(pool, meta, k_out, v_out, table, step, window, nkv, hd) -> 
 
 
 @functools.lru_cache(maxsize=4096)
-def kv4_attend_plan(n_seqs: int, nkv: int, cols: int, pages: int) -> tuple:
+def kv4_attend_plan(n_seqs: int, nkv: int, hd: int, cols: int, pages: int) -> tuple:
     """(tiles of eight columns a CTA takes, pages per chunk, chunks) for ``kv4_attend``: ``cols`` query columns (heads of a kv head
     times tokens) of the sequence with the most, ``pages`` of keys that the longest sequence's tokens see.
 
-    By rounds of the CTAs that find room (four of an SM with eight columns, two with sixteen) times what one takes: its pages and about three
-    more for setting up and joining its warps' sums; the chunks' joining costs two and a third of one per chunk. Measured (us, as
+    By rounds of the CTAs that find room (four of an SM with eight columns, two with sixteen, three of heads up to 64) times what one takes:
+    its pages and about three more for setting up and joining its warps' sums; the chunks' joining costs two and a third of one per chunk. Measured (us, as
     chosen / otherwise): 64 sequences of 2,048 keys 50 in one chunk, 52 in two, 56 in four; 3 of about 50,000 71 in 24, 77 in 16, 81 in
-    32; one of 2,048 10.7 in eleven, 10.3 in seven, 12.3 in seventeen; 40 tokens behind 6,000 46 in three, 52 in six."""
+    32; one of 2,048 10.7 in eleven, 10.3 in seven, 12.3 in seventeen; 40 tokens behind 6,000 46 in three, 52 in six; with
+    heads of 64 31 in five, 36 in three."""
     nt = 1 if cols <= 8 else 2
-    base, room = n_seqs * nkv * -(-cols // (8 * nt)), 592 if nt == 1 else 296
+    base, room = n_seqs * nkv * -(-cols // (8 * nt)), 592 if nt == 1 else 296 if hd > 64 else 444
     best = None
     for n in range(1, min(pages, max(1, 2 * room // base)) + 1):
         each = -(-pages // n)
@@ -2009,7 +2010,7 @@ def kv4_attend(q, pool, out, meta, seq_start, n_seqs: int, max_new: int, longest
     pages = -(-longest // 64)
     if window:
         pages = min(pages, (window + max_new - 2) // 64 + 2)
-    nt, chunk_pages, n_chunks = plan or kv4_attend_plan(n_seqs, nkv, max_new * (nh // nkv), max(1, pages))
+    nt, chunk_pages, n_chunks = plan or kv4_attend_plan(n_seqs, nkv, hd, max_new * (nh // nkv), max(1, pages))
     need = T * nh * n_chunks * (hd + 2) if n_chunks > 1 else 0
     scratch = torch.empty(need, dtype=torch.float32, device=q.device) if need else None
     if _RANGE_CHECKED["kv4_attention"]:

@@ -44,7 +44,7 @@ def length_bucket(max_len: int, page_size: int) -> int:
 
 
 FLASH_TC_TOKENS = 256      # bfloat16 prompt steps of at least so many tokens take the tcgen05 attention
-SPLIT4_COLUMNS = 256       # prompt steps of up to so many query columns (tokens x heads of a kv head) read a four-bit cache as it lies
+SPLIT4_COLUMNS = 256       # bfloat16 prompt steps of up to so many query columns (tokens x heads of a kv head) of a sequence read a four-bit cache as it lies
 TILED_TOKENS = 32          # 32-bit prompt steps of at least so many tokens take the attention kernel of 64-query tiles
 
 
@@ -225,6 +225,17 @@ def attend_paged(q, step, cache, nh, nkv, hd, window, scale, sink=None, counters
     return ctx
 
 
+def reads_codes(q, cols: int, nkv: int) -> bool:
+    """Whether a prompt step's attention works on the codes of a four-bit cache, or on its pages unpacked first. ``cols``: the most
+    query columns of a sequence. On the codes every 16 columns take a page apart again; unpacked, short steps meet the tile
+    kernels, which take a sequence's keys one after another. Measured, us (codes / unpacked first), 32 heads on 8 of 128:
+      bfloat16, tokens behind 2,000: 64 32/75, 192 80/81, 256 94/59, 1,024 358/78; 1,024 tokens of 64 sequences behind 1,000 172/286;
+      float32, tokens behind nothing: 64 10/28, 512 58/148, 2,000 434/1,490; 512 behind 2,000 243/961."""
+    if q.dtype == torch.float32:
+        return nkv * -(-cols // 16) < 1 << 16            # (tiles of columns are a grid's second dimension)
+    return q.shape[0] < FLASH_TC_TOKENS or cols <= SPLIT4_COLUMNS
+
+
 def attend_four_bits(q, step, cache, nh, nkv, hd, window, scale, sink=None):
     """``attend_paged`` over pages of four bits."""
     T = q.shape[0]
@@ -232,7 +243,7 @@ def attend_four_bits(q, step, cache, nh, nkv, hd, window, scale, sink=None):
         raise K.KernelError(f"attention: queries are [tokens, {nh} x {hd}], bfloat16 or float32, of heads in equal groups")
     if not scale > 0:
         raise K.KernelError(f"attention over a four-bit cache takes a positive scale, got {scale}")
-    if step.all_single or step.max_new * (nh // nkv) <= SPLIT4_COLUMNS:
+    if step.all_single or reads_codes(q, step.max_new * (nh // nkv), nkv):
         out = torch.empty_like(q)
         # (a decode step by its length's bucket, as below: run directly and replayed from a graph it adds up in the same order)
         longest = length_bucket(step.max_len, cache.page_size) if step.all_single else step.max_len
