@@ -20,6 +20,10 @@
 // A page of a kv head is one run of bytes and arrives by one bulk copy in a ring; four warps take 16 of its keys each and keep
 // sums of their own, joined at the end in the order of the warps, then of the chunks: results do not depend on timing.
 // A key or value that is not finite reaches the columns that see it and no others.
+//
+// Measured (32 heads on 8 of 128, bfloat16): 64 sequences of 2,048 keys 50 us for 122 MB of pages, 2.4 TB/s; 3 of about 60,000 73;
+// 40 tokens behind 6,000 47; one sequence of 2,048 with heads of 64 10.7. Bound by instructions: some 470 a warp for 16 keys and eight
+// columns, with 57 % of the issue slots used at 64 sequences; more CTAs an SM (five of eight columns, three of sixteen) gain nothing.
 #include "kv4.cuh"
 #include "async_copy.cuh"
 #include <cuda_fp16.h>
