@@ -275,6 +275,8 @@ def check4(lin, x, out, out_features: int, accumulate: bool) -> int:
         raise K.KernelError(f"shapes do not match: x {tuple(x.shape)}, weight [{out_features}, {lin.in_features}], out {tuple(out.shape)}")
     if x.stride(1) != 1 or out.stride(1) != 1:
         raise K.KernelError("product operands must have unit stride in their last dimension")
+    if x.shape[0] > 1 and out.stride(0) < out_features:
+        raise K.KernelError("the rows of a product's output may not overlap")
     if not (x.get_device() == out.get_device() == lin.codes.get_device() == torch._C._cuda_getDevice()):
         raise K.KernelError(f"the weight (on {lin.codes.device}), its rows and its output live on the current device, got {x.device} and {out.device}")
     return x.shape[0]

@@ -102,6 +102,15 @@ def test_rows_that_overlap_and_rows_of_nothing():
         assert bool((zero == 0).all())
 
 
+def test_an_outputs_rows_that_overlap_are_refused():
+    from spissa_b200.csrc.lib import KernelError
+    from spissa_b200.parts.linear import Linear4
+    lin = Linear4(numbers(48, 128, seed=2, dtype=BF).to(DEV), 32)
+    for M in (2, 20):
+        with pytest.raises(KernelError):
+            lin(torch.zeros(M, 128, dtype=BF, device=DEV), out=torch.zeros(1, 48, device=DEV).expand(M, 48))
+
+
 def test_products_on_another_stream_and_in_graphs():
     from spissa_b200.parts.linear import GatedLinear4, Linear4
     w = numbers(512, 1024, seed=4, spread=0.5, dtype=BF).to(DEV)
@@ -204,6 +213,37 @@ def test_prompts_behind_a_window_meet_no_memory_that_was_left_alone(dtype):
         out = run_attention(meta, pool, q, nh, nkv, hd, window, None, new, before)
         # (keys and values are exact in the queries' type; the bfloat16 kernels round probabilities once, as counted)
         assert bool(((out.cpu().double() - want).abs() <= 2 * tol).all())
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("window", [1, 2, 64, 65, 128])
+def test_windows_at_the_borders_of_pages(window, dtype):
+    nh, nkv, hd = 6, 2, 64
+    for new, before in (([1, 1, 1], [63, 64, 191]), ([5, 1, 40], [60, 0, 100]), ([280], [70])):
+        meta, kv, q, sinks, want, mag, span = attention_case(nh, nkv, hd, dtype, new, before, window, 70 + window, window == 64)
+        out = run_attention(meta, fill(meta, kv, nkv, hd), q, nh, nkv, hd, window, sinks, new, before)
+        assert bool(((out.cpu().double() - want).abs() <= attention_tolerance(hd, dtype, want, mag, span)).all())
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("nh,nkv,hd", [(8, 2, 128), (9, 3, 96), (4, 2, 32), (16, 2, 64)])
+def test_prompts_on_the_codes_and_unpacked_first_agree(nh, nkv, hd, dtype, monkeypatch):
+    """Whichever way a step would take by its sizes, both give what the definition gives."""
+    from spissa_b200.parts import attention as A
+    for new, before in (([70, 1, 30], [10, 500, 0]), ([300], [65])):
+        meta, kv, q, sinks, want, mag, span = attention_case(nh, nkv, hd, dtype, new, before, None, 80 + hd, True)
+        pool = fill(meta, kv, nkv, hd)
+        for codes in (True, False):
+            monkeypatch.setattr(A, "reads_codes", lambda *a: codes)
+            out = run_attention(meta, pool, q, nh, nkv, hd, None, sinks, new, before)
+            assert bool(((out.cpu().double() - want).abs() <= attention_tolerance(hd, dtype, want, mag, span)).all()), codes
+
+
+def test_the_way_of_a_prompt_step():
+    from spissa_b200.parts.attention import reads_codes
+    q = torch.empty(255, 8, dtype=BF, device=DEV)
+    assert reads_codes(q, 1020, 8) and not reads_codes(q.new_empty(256, 8), 1024, 8) and reads_codes(q.new_empty(1024, 8), 256, 8)
+    assert reads_codes(q.float(), 1 << 16, 8) and not reads_codes(q.float(), 1 << 18, 8)
 
 
 def test_a_pool_beyond_four_gigabytes():
