@@ -126,7 +126,6 @@ template <typename TQ, int NG, int NT>
 __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 2)
 attend_kernel(const Args a) {
     constexpr int HD = 32 * NG, PARTS = sizeof(TQ) == 4 ? 2 : 1, COLS = 8 * NT, TILE = kv4_tile_bytes(HD), MW = (NG + 1) / 2;
-    constexpr int PP = 1;
     constexpr bool Q_HELD = NT == 1 && PARTS == 1;                   // the queries' operands in registers, else in shared memory
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES];
@@ -250,7 +249,7 @@ attend_kernel(const Args a) {
         for (int e = 0; e < 2; ++e) { sum[n][e] = 0.0f; ref[n][e] = 0.0f; top[n][e] = limit[n][e] = -INFINITY; }
     }
 
-    for (int it = 0; it < n_pages; it += PP) {
+    for (int it = 0; it < n_pages; ++it) {
         // the stage that every warp had done with a page ago gets the next page
         if (warp == 0 && it > 0 && it - 1 + STAGES < n_pages) {
             const int i = it - 1 + STAGES;
@@ -259,108 +258,98 @@ attend_kernel(const Args a) {
             if (lane == 0 && mbar_wait_flag(smem_u32(&empty[(it - 1) % STAGES]), ((it - 1) / STAGES) & 1, a.status, 141, &failed)) fetch(i, page);
         }
         __syncwarp();
-        float x[PP][NT][4];
-        uint32_t m0[PP][MW], m1[PP][MW];                             // the values' scales of this lane's two keys of a page
+        mbar_wait_flag(smem_u32(&full[it % STAGES]), (it / STAGES) & 1, a.status, 142, &failed);
+        const int page_pos = (page0 + it) * KV4_PAGE;
+        const uint32_t at = ring + (it % STAGES) * TILE;
+        const int r0 = warp * 16 + g;                            // rows of the page's keys as they lie: this lane's are r0 and r0 + 8
+        const int p0 = warp * 16 + (g & 1) * 4 + (g >> 1), key = page_pos + p0;        // their positions: this and 8 on
+        float x[NT][4];
+        uint32_t m0[MW], m1[MW];                                     // the values' scales of this lane's two keys
+        // scores of 16 keys: rows g and g + 8, columns 2 t and 2 t + 1
 #pragma unroll
-        for (int j = 0; j < PP; ++j) {
-            const bool here = it + j < n_pages;                      // (the last turn may lack a page: nobody sees its keys)
-            if (here) mbar_wait_flag(smem_u32(&full[(it + j) % STAGES]), ((it + j) / STAGES) & 1, a.status, 142, &failed);
-            const int page_pos = (page0 + it + j) * KV4_PAGE;
-            const uint32_t at = ring + ((it + j) % STAGES) * TILE;
-            const int r0 = warp * 16 + g;                            // rows of the page's keys as they lie: this lane's are r0 and r0 + 8
-            const int p0 = warp * 16 + (g & 1) * 4 + (g >> 1), key = page_pos + p0;        // their positions: this and 8 on
-            // scores of 16 keys: rows g and g + 8, columns 2 t and 2 t + 1
+        for (int n = 0; n < NT; ++n) x[n][0] = x[n][1] = x[n][2] = x[n][3] = 0.0f;
+        uint32_t k0[NG], k1[NG], km0[MW], km1[MW];
+        lds_words<NG>(at + r0 * (HD / 2) + t * (NG * 4), k0);
+        lds_words<NG>(at + (r0 + 8) * (HD / 2) + t * (NG * 4), k1);
+        lds_halves<NG>(at + kv4_k_meta(HD) + r0 * (NG * 2), km0);
+        lds_halves<NG>(at + kv4_k_meta(HD) + (r0 + 8) * (NG * 2), km1);
+        lds_halves<NG>(at + kv4_v_meta(HD) + p0 * (NG * 2), m0);
+        lds_halves<NG>(at + kv4_v_meta(HD) + (p0 + 8) * (NG * 2), m1);
 #pragma unroll
-            for (int n = 0; n < NT; ++n) x[j][n][0] = x[j][n][1] = x[j][n][2] = x[j][n][3] = 0.0f;
-            uint32_t k0[NG], k1[NG], km0[MW], km1[MW];
-            lds_words<NG>(at + r0 * (HD / 2) + t * (NG * 4), k0);
-            lds_words<NG>(at + (r0 + 8) * (HD / 2) + t * (NG * 4), k1);
-            lds_halves<NG>(at + kv4_k_meta(HD) + r0 * (NG * 2), km0);
-            lds_halves<NG>(at + kv4_k_meta(HD) + (r0 + 8) * (NG * 2), km1);
-            lds_halves<NG>(at + kv4_v_meta(HD) + p0 * (NG * 2), m0[j]);
-            lds_halves<NG>(at + kv4_v_meta(HD) + (p0 + 8) * (NG * 2), m1[j]);
+        for (int i = 0; i < NG; ++i) {
+            const float s0 = scale_at(km0, i), s1 = scale_at(km1, i), z0 = zero_at(km0, i), z1 = zero_at(km1, i);
+            const uint32_t u0 = k0[i], u1 = k1[i], w0 = u0 >> 8, w1 = u1 >> 8;
+            uint32_t c[8] = {u0 & 0x000f000fu, u1 & 0x000f000fu, u0 & 0x00f000f0u, u1 & 0x00f000f0u, w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u};
+            if (PARTS == 2) {
+                const uint32_t y0 = ((km0[i >> 1] >> (16 * (i & 1))) & 15u) * 0x10001u, y1 = ((km1[i >> 1] >> (16 * (i & 1))) & 15u) * 0x10001u;
 #pragma unroll
-            for (int i = 0; i < NG; ++i) {
-                const float s0 = scale_at(km0, i), s1 = scale_at(km1, i), z0 = zero_at(km0, i), z1 = zero_at(km1, i);
-                const uint32_t u0 = k0[i], u1 = k1[i], w0 = u0 >> 8, w1 = u1 >> 8;
-                uint32_t c[8] = {u0 & 0x000f000fu, u1 & 0x000f000fu, u0 & 0x00f000f0u, u1 & 0x00f000f0u, w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u};
-                if (PARTS == 2) {
-                    const uint32_t y0 = ((km0[i >> 1] >> (16 * (i & 1))) & 15u) * 0x10001u, y1 = ((km1[i >> 1] >> (16 * (i & 1))) & 15u) * 0x10001u;
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) c[k] = q4_less(c[k], (k & 1 ? y1 : y0) << (k & 2 ? 4 : 0));
-                }
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    float acc[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int part = PARTS - 1; part >= 0; --part) {
-                        uint4 qv;
-                        if (Q_HELD) qv = make_uint4(qh[Q_HELD ? i : 0][0], qh[Q_HELD ? i : 0][1], qh[Q_HELD ? i : 0][2], qh[Q_HELD ? i : 0][3]);
-                        else qv = lds16(q_at + (uint32_t)(((n * NG + i) * PARTS + part) * 32 + lane) * 16);
-                        mma_f16(acc, c[0], c[1], c[2], c[3], qv.x, qv.y);
-                        mma_f16(acc, c[4], c[5], c[6], c[7], qv.z, qv.w);
-                    }
-                    float (&y)[4] = x[j][n];
-                    if (PARTS == 2) {
-                        y[0] = fmaf(s0, acc[0], y[0]);
-                        y[1] = fmaf(s0, acc[1], y[1]);
-                        y[2] = fmaf(s1, acc[2], y[2]);
-                        y[3] = fmaf(s1, acc[3], y[3]);
-                        continue;
-                    }
-                    y[0] = fmaf(s0, fmaf(z0, qs[n][i][0], acc[0]), y[0]);
-                    y[1] = fmaf(s0, fmaf(z0, qs[n][i][1], acc[1]), y[1]);
-                    y[2] = fmaf(s1, fmaf(z1, qs[n][i][0], acc[2]), y[2]);
-                    y[3] = fmaf(s1, fmaf(z1, qs[n][i][1], acc[3]), y[3]);
-                }
+                for (int k = 0; k < 8; ++k) c[k] = q4_less(c[k], (k & 1 ? y1 : y0) << (k & 2 ? 4 : 0));
             }
-            if (!here || page_pos + KV4_PAGE - 1 > first_pos || (a.window && page_pos < last_pos + 1 - a.window)) {       // not all of it is seen by all
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
+            for (int n = 0; n < NT; ++n) {
+                float acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int p = pos[n][e & 1], k = key + (e & 2) * 4;
-                        if (!here || k > p || (a.window && k <= p - a.window)) x[j][n][e] = -INFINITY;
-                    }
-#pragma unroll
-                for (int i = 0; i < MW; ++i) {                       // what nobody sees may be anything
-                    if (!here || key > last_pos || key < lowest) m0[j][i] = 0;
-                    if (!here || key + 8 > last_pos || key + 8 < lowest) m1[j][i] = 0;
+                for (int part = PARTS - 1; part >= 0; --part) {
+                    uint4 qv;
+                    if (Q_HELD) qv = make_uint4(qh[Q_HELD ? i : 0][0], qh[Q_HELD ? i : 0][1], qh[Q_HELD ? i : 0][2], qh[Q_HELD ? i : 0][3]);
+                    else qv = lds16(q_at + (uint32_t)(((n * NG + i) * PARTS + part) * 32 + lane) * 16);
+                    mma_f16(acc, c[0], c[1], c[2], c[3], qv.x, qv.y);
+                    mma_f16(acc, c[4], c[5], c[6], c[7], qv.z, qv.w);
                 }
+                float (&y)[4] = x[n];
+                if (PARTS == 2) {
+                    y[0] = fmaf(s0, acc[0], y[0]);
+                    y[1] = fmaf(s0, acc[1], y[1]);
+                    y[2] = fmaf(s1, acc[2], y[2]);
+                    y[3] = fmaf(s1, acc[3], y[3]);
+                    continue;
+                }
+                y[0] = fmaf(s0, fmaf(z0, qs[n][i][0], acc[0]), y[0]);
+                y[1] = fmaf(s0, fmaf(z0, qs[n][i][1], acc[1]), y[1]);
+                y[2] = fmaf(s1, fmaf(z1, qs[n][i][0], acc[2]), y[2]);
+                y[3] = fmaf(s1, fmaf(z1, qs[n][i][1], acc[3]), y[3]);
+            }
+        }
+        if (page_pos + KV4_PAGE - 1 > first_pos || (a.window && page_pos < last_pos + 1 - a.window)) {       // not all of it is seen by all
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int p = pos[n][e & 1], k = key + (e & 2) * 4;
+                    if (k > p || (a.window && k <= p - a.window)) x[n][e] = -INFINITY;
+                }
+#pragma unroll
+            for (int i = 0; i < MW; ++i) {                       // what nobody sees may be anything
+                if (key > last_pos || key < lowest) m0[i] = 0;
+                if (key + 8 > last_pos || key + 8 < lowest) m1[i] = 0;
             }
         }
         // do the references hold?
         uint32_t most = s_bits;
         bool moves = false;
 #pragma unroll
-        for (int j = 0; j < PP; ++j) {
+        for (int i = 0; i < MW; ++i) most = __vmaxu2(most, __vmaxu2(m0[i], m1[i]));
 #pragma unroll
-            for (int i = 0; i < MW; ++i) most = __vmaxu2(most, __vmaxu2(m0[j][i], m1[j][i]));
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) moves |= x[j][n][e] > limit[n][e & 1];
-        }
+            for (int e = 0; e < 4; ++e) moves |= x[n][e] > limit[n][e & 1];
         if (__any_sync(0xffffffffu, moves || most != s_bits)) {
             // scales that are not numbers: noted for the columns that see their keys, and taken as zero
             most = 0;
 #pragma unroll
-            for (int j = 0; j < PP; ++j) {
+            for (int i = 0; i < NG; ++i) {
+                const int sh = 16 * (i & 1);
+                const bool bad0 = ((m0[i >> 1] >> sh) & 0x7f80u) == 0x7f80u, bad1 = ((m1[i >> 1] >> sh) & 0x7f80u) == 0x7f80u;
 #pragma unroll
-                for (int i = 0; i < NG; ++i) {
-                    const int sh = 16 * (i & 1);
-                    const bool bad0 = ((m0[j][i >> 1] >> sh) & 0x7f80u) == 0x7f80u, bad1 = ((m1[j][i >> 1] >> sh) & 0x7f80u) == 0x7f80u;
+                for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int n = 0; n < NT; ++n)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e)
-                            if ((bad0 && x[j][n][e] != -INFINITY) || (bad1 && x[j][n][2 + e] != -INFINITY)) poison[n] |= 1u << (2 * i + e);
-                    if (bad0) m0[j][i >> 1] &= ~(0xffffu << sh);
-                    if (bad1) m1[j][i >> 1] &= ~(0xffffu << sh);
-                }
-#pragma unroll
-                for (int i = 0; i < MW; ++i) most = __vmaxu2(most, __vmaxu2(m0[j][i], m1[j][i]));
+                    for (int e = 0; e < 2; ++e)
+                        if ((bad0 && x[n][e] != -INFINITY) || (bad1 && x[n][2 + e] != -INFINITY)) poison[n] |= 1u << (2 * i + e);
+                if (bad0) m0[i >> 1] &= ~(0xffffu << sh);
+                if (bad1) m1[i >> 1] &= ~(0xffffu << sh);
             }
+#pragma unroll
+            for (int i = 0; i < MW; ++i) most = __vmaxu2(most, __vmaxu2(m0[i], m1[i]));
             most = max(most & 0xffffu, most >> 16) | 15u;             // (with every zero: what is compared is the whole half word)
             s_bits = max(s_bits & 0xffffu, __reduce_max_sync(0xffffffffu, most)) * 0x10001u;
             const float s_top = __uint_as_float((s_bits & 0xfff0u) << 16);
@@ -370,9 +359,7 @@ attend_kernel(const Args a) {
                 float f[2];
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    float big = fmaxf(x[0][n][e], x[0][n][2 + e]);
-#pragma unroll
-                    for (int j = 1; j < PP; ++j) big = fmaxf(big, fmaxf(x[j][n][e], x[j][n][2 + e]));
+                    float big = fmaxf(x[n][e], x[n][2 + e]);
                     big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 4));
                     big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 8));
                     big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 16));
@@ -397,71 +384,63 @@ attend_kernel(const Args a) {
             }
         }
 #pragma unroll
-        for (int j = 0; j < PP; ++j) {
-            const uint32_t at = ring + ((it + j) % STAGES) * TILE;
-            float (&y)[NT][4] = x[j];
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[n][e] = ex2(fmaf(x[n][e], unit[n][e & 1], -ref[n][e & 1]));
+            sum[n][0] += x[n][0] + x[n][2];
+            sum[n][1] += x[n][1] + x[n][3];
+        }
+        // the output of 16 keys
+        uint32_t v[4][MW], mz[PARTS == 2 ? 4 : 1][MW];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int p = warp * 16 + 4 * k + t, sw = HD == 128 ? (p & 2) << 4 : 0;
+            lds_halves<NG>(at + kv4_v_codes(HD) + p * (HD / 2) + ((g * NG * 2) ^ sw), v[k]);
+            if (PARTS == 2) lds_halves<NG>(at + kv4_v_meta(HD) + p * (NG * 2), mz[PARTS == 2 ? k : 0]);
+        }
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+            const float s0 = scale_at(m0, i), s1 = scale_at(m1, i);
+            const int half = i & 1 ? 0x7632 : 0x5410;
+            // keys t, 4 + t and 8 + t, 12 + t side by side
+            const uint32_t u0 = __byte_perm(v[0][i >> 1], v[1][i >> 1], half), u1 = __byte_perm(v[2][i >> 1], v[3][i >> 1], half);
+            const uint32_t w0 = u0 >> 8, w1 = u1 >> 8;
+            uint32_t c[8] = {u0 & 0x000f000fu, u0 & 0x00f000f0u, u1 & 0x000f000fu, u1 & 0x00f000f0u, w0 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x000f000fu, w1 & 0x00f000f0u};
+            if (PARTS == 2) {
+                const uint32_t y0 = __byte_perm(mz[0][i >> 1], mz[PARTS == 2 ? 1 : 0][i >> 1], half) & 0x000f000fu;
+                const uint32_t y1 = __byte_perm(mz[PARTS == 2 ? 2 : 0][i >> 1], mz[PARTS == 2 ? 3 : 0][i >> 1], half) & 0x000f000fu;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) c[k] = q4_less(c[k], (k & 2 ? y1 : y0) << (k & 1 ? 4 : 0));
+            }
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) y[n][e] = ex2(fmaf(y[n][e], unit[n][e & 1], -ref[n][e & 1]));
-                sum[n][0] += y[n][0] + y[n][2];
-                sum[n][1] += y[n][1] + y[n][3];
-            }
-            // the output of 16 keys
-            uint32_t v[4][MW], mz[PARTS == 2 ? 4 : 1][MW];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int p = warp * 16 + 4 * k + t, sw = HD == 128 ? (p & 2) << 4 : 0;
-                lds_halves<NG>(at + kv4_v_codes(HD) + p * (HD / 2) + ((g * NG * 2) ^ sw), v[k]);
-                if (PARTS == 2) lds_halves<NG>(at + kv4_v_meta(HD) + p * (NG * 2), mz[PARTS == 2 ? k : 0]);
-            }
-#pragma unroll
-            for (int i = 0; i < NG; ++i) {
-                const float s0 = scale_at(m0[j], i), s1 = scale_at(m1[j], i);
-                const int half = i & 1 ? 0x7632 : 0x5410;
-                // keys t, 4 + t and 8 + t, 12 + t side by side
-                const uint32_t u0 = __byte_perm(v[0][i >> 1], v[1][i >> 1], half), u1 = __byte_perm(v[2][i >> 1], v[3][i >> 1], half);
-                const uint32_t w0 = u0 >> 8, w1 = u1 >> 8;
-                uint32_t c[8] = {u0 & 0x000f000fu, u0 & 0x00f000f0u, u1 & 0x000f000fu, u1 & 0x00f000f0u, w0 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x000f000fu, w1 & 0x00f000f0u};
+                const float p0 = x[n][0] * s0, p1 = x[n][1] * s0, p2 = x[n][2] * s1, p3 = x[n][3] * s1;
+                const uint32_t h0 = half2_of(p0, p1), h1 = half2_of(p2, p3), b0 = transposed(h0), b1 = transposed(h1);
                 if (PARTS == 2) {
-                    const uint32_t y0 = __byte_perm(mz[0][i >> 1], mz[PARTS == 2 ? 1 : 0][i >> 1], half) & 0x000f000fu;
-                    const uint32_t y1 = __byte_perm(mz[PARTS == 2 ? 2 : 0][i >> 1], mz[PARTS == 2 ? 3 : 0][i >> 1], half) & 0x000f000fu;
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) c[k] = q4_less(c[k], (k & 2 ? y1 : y0) << (k & 1 ? 4 : 0));
-                }
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    const float p0 = y[n][0] * s0, p1 = y[n][1] * s0, p2 = y[n][2] * s1, p3 = y[n][3] * s1;
-                    const uint32_t h0 = half2_of(p0, p1), h1 = half2_of(p2, p3), b0 = transposed(h0), b1 = transposed(h1);
-                    if (PARTS == 2) {
-                        // sums of a page of their own, added in 32 bits: the tensor cores' own additions cut instead of rounding
-                        const float2 f0 = __half22float2(*(const __half2*)&h0), f1 = __half22float2(*(const __half2*)&h1);
-                        const uint32_t l0 = transposed(half2_of(p0 - f0.x, p1 - f0.y)), l1 = transposed(half2_of(p2 - f1.x, p3 - f1.y));
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            float o[4] = {0.f, 0.f, 0.f, 0.f};
-                            mma_f16(o, c[4 * h], c[4 * h + 1], c[4 * h + 2], c[4 * h + 3], l0, l1);
-                            mma_f16(o, c[4 * h], c[4 * h + 1], c[4 * h + 2], c[4 * h + 3], b0, b1);
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) O[n][i][h][e] += o[e];
-                        }
-                        continue;
-                    }
-                    mma_f16(O[n][i][0], c[0], c[1], c[2], c[3], b0, b1);
-                    mma_f16(O[n][i][1], c[4], c[5], c[6], c[7], b0, b1);
-                    // (the zeros are taken off with the same rounded numbers, so that a value of zero adds exactly nothing)
-                    const float z0 = zero_at(m0[j], i), z1 = zero_at(m1[j], i);
+                    // sums of a page of their own, added in 32 bits: the tensor cores' own additions cut instead of rounding
                     const float2 f0 = __half22float2(*(const __half2*)&h0), f1 = __half22float2(*(const __half2*)&h1);
-                    zs[n][i][0] = fmaf(f0.x, z0, fmaf(f1.x, z1, zs[n][i][0]));
-                    zs[n][i][1] = fmaf(f0.y, z0, fmaf(f1.y, z1, zs[n][i][1]));
+                    const uint32_t l0 = transposed(half2_of(p0 - f0.x, p1 - f0.y)), l1 = transposed(half2_of(p2 - f1.x, p3 - f1.y));
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        float o[4] = {0.f, 0.f, 0.f, 0.f};
+                        mma_f16(o, c[4 * h], c[4 * h + 1], c[4 * h + 2], c[4 * h + 3], l0, l1);
+                        mma_f16(o, c[4 * h], c[4 * h + 1], c[4 * h + 2], c[4 * h + 3], b0, b1);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) O[n][i][h][e] += o[e];
+                    }
+                    continue;
                 }
+                mma_f16(O[n][i][0], c[0], c[1], c[2], c[3], b0, b1);
+                mma_f16(O[n][i][1], c[4], c[5], c[6], c[7], b0, b1);
+                // (the zeros are taken off with the same rounded numbers, so that a value of zero adds exactly nothing)
+                const float z0 = zero_at(m0, i), z1 = zero_at(m1, i);
+                const float2 f0 = __half22float2(*(const __half2*)&h0), f1 = __half22float2(*(const __half2*)&h1);
+                zs[n][i][0] = fmaf(f0.x, z0, fmaf(f1.x, z1, zs[n][i][0]));
+                zs[n][i][1] = fmaf(f0.y, z0, fmaf(f1.y, z1, zs[n][i][1]));
             }
         }
         __syncwarp();
-        if (lane == 0)
-#pragma unroll
-            for (int j = 0; j < PP; ++j)
-                if (it + j < n_pages) mbar_arrive(smem_u32(&empty[(it + j) % STAGES]));
+        if (lane == 0) mbar_arrive(smem_u32(&empty[it % STAGES]));
     }
 
     // each warp's sums over its lanes, its columns' numbers in shared memory (where the pages were); then the warps', in their order
