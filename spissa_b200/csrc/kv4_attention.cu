@@ -10,10 +10,12 @@
 // its columns: nothing is wasted on padding up to eight heads. Scales and zeros are applied to what is small:
 //   score  Σ_groups s (Σ q' c − z Σ q'), q' = q times a power of two that brings a head's largest entry to 2^14 (exact for
 //          bfloat16; float32 as two float16 parts, 22 bits);
-//   output Σ_keys (p s) c − Σ_keys (p s) z: p s is rounded to float16 (2^-12 of itself; float32: two parts, 2^-23) under a
-//          reference that holds it below 2^15, so that the scale s of a key's group of values costs no rounding of the values.
-// With float32 queries the operands are c − z itself (1024 + c less 1024 + z), and a page's sums are added in 32 bits: tensor
-// cores cut partial sums to 24 bits, and sums of p s c are many times those of p s (c − z).
+//   output Σ_keys (p s) (c − z): p s is rounded to float16 (2^-11 of itself; float32: two parts, 2^-22) under a reference
+//          that holds it below 2^15, so that the scale s of a key's group of values costs no rounding of the values.
+// The output's operands are c − z, differences of two such numbers, which are exact: tensor cores cut partial sums to 24 bits, and sums of
+// p s c are many times those of p s (c − z), which are nothing where the values are zeros. (With z Σ p s taken off at the end a value of
+// zero came to 2^-24 of 15 s a page. 64 sequences of 2,048 keys: 50.3 us so, 51.0 now; 40 tokens behind 6,000: 46.2 and 44.6.) With
+// float32 queries the scores' operands are c − z too, as 1024 + c less 1024 + z, and a page's sums are added in 32 bits.
 // The reference of a column follows its largest score, and the largest scale of the values, in steps: it moves only when a
 // score passes it by more than 2^8 or a scale passes the one it was made for; then the sums are multiplied by a power of two.
 //
@@ -72,6 +74,11 @@ __device__ __forceinline__ uint32_t transposed(uint32_t v) {          // of an 8
 __device__ __forceinline__ uint32_t half2_of(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *(const uint32_t*)&h;
+}
+// of two pairs of float16 numbers, subnormal ones as any other
+__device__ __forceinline__ uint32_t half2_less(uint32_t a, uint32_t b) {
+    const __half2 r = __hsub2(*(const __half2*)&a, *(const __half2*)&b);
+    return *(const uint32_t*)&r;
 }
 __device__ __forceinline__ uint4 lds16(uint32_t at) {
     uint4 v;
@@ -233,18 +240,16 @@ attend_kernel(const Args a) {
     if (!Q_HELD) __syncthreads();
 
     // top: the score (log2, rounded up) that a column's reference was made for; limit: how far a raw score may go under it
-    float O[NT][NG][2][4], zs[NT][NG][2], sum[NT][2], ref[NT][2], top[NT][2], limit[NT][2];
+    float O[NT][NG][2][4], sum[NT][2], ref[NT][2], top[NT][2], limit[NT][2];
     uint32_t poison[NT];
     uint32_t s_bits = 0;                                             // the largest scale the references were made for, twice, zeros of 15
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         poison[n] = 0;
 #pragma unroll
-        for (int i = 0; i < NG; ++i) {
-            zs[n][i][0] = zs[n][i][1] = 0.0f;
+        for (int i = 0; i < NG; ++i)
 #pragma unroll
             for (int h = 0; h < 2; ++h) O[n][i][h][0] = O[n][i][h][1] = O[n][i][h][2] = O[n][i][h][3] = 0.0f;
-        }
 #pragma unroll
         for (int e = 0; e < 2; ++e) { sum[n][e] = 0.0f; ref[n][e] = 0.0f; top[n][e] = limit[n][e] = -INFINITY; }
     }
@@ -375,12 +380,9 @@ attend_kernel(const Args a) {
                     sum[n][e] *= f[e];
                 }
 #pragma unroll
-                for (int i = 0; i < NG; ++i) {
+                for (int i = 0; i < NG; ++i)
 #pragma unroll
                     for (int h = 0; h < 2; ++h) { O[n][i][h][0] *= f[0]; O[n][i][h][1] *= f[1]; O[n][i][h][2] *= f[0]; O[n][i][h][3] *= f[1]; }
-                    zs[n][i][0] *= f[0];
-                    zs[n][i][1] *= f[1];
-                }
             }
         }
 #pragma unroll
@@ -391,12 +393,12 @@ attend_kernel(const Args a) {
             sum[n][1] += x[n][1] + x[n][3];
         }
         // the output of 16 keys
-        uint32_t v[4][MW], mz[PARTS == 2 ? 4 : 1][MW];
+        uint32_t v[4][MW], mz[4][MW];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const int p = warp * 16 + 4 * k + t, sw = HD == 128 ? (p & 2) << 4 : 0;
             lds_halves<NG>(at + kv4_v_codes(HD) + p * (HD / 2) + ((g * NG * 2) ^ sw), v[k]);
-            if (PARTS == 2) lds_halves<NG>(at + kv4_v_meta(HD) + p * (NG * 2), mz[PARTS == 2 ? k : 0]);
+            lds_halves<NG>(at + kv4_v_meta(HD) + p * (NG * 2), mz[k]);
         }
 #pragma unroll
         for (int i = 0; i < NG; ++i) {
@@ -406,12 +408,9 @@ attend_kernel(const Args a) {
             const uint32_t u0 = __byte_perm(v[0][i >> 1], v[1][i >> 1], half), u1 = __byte_perm(v[2][i >> 1], v[3][i >> 1], half);
             const uint32_t w0 = u0 >> 8, w1 = u1 >> 8;
             uint32_t c[8] = {u0 & 0x000f000fu, u0 & 0x00f000f0u, u1 & 0x000f000fu, u1 & 0x00f000f0u, w0 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x000f000fu, w1 & 0x00f000f0u};
-            if (PARTS == 2) {
-                const uint32_t y0 = __byte_perm(mz[0][i >> 1], mz[PARTS == 2 ? 1 : 0][i >> 1], half) & 0x000f000fu;
-                const uint32_t y1 = __byte_perm(mz[PARTS == 2 ? 2 : 0][i >> 1], mz[PARTS == 2 ? 3 : 0][i >> 1], half) & 0x000f000fu;
+            const uint32_t y0 = __byte_perm(mz[0][i >> 1], mz[1][i >> 1], half) & 0x000f000fu, y1 = __byte_perm(mz[2][i >> 1], mz[3][i >> 1], half) & 0x000f000fu;
 #pragma unroll
-                for (int k = 0; k < 8; ++k) c[k] = q4_less(c[k], (k & 2 ? y1 : y0) << (k & 1 ? 4 : 0));
-            }
+            for (int k = 0; k < 8; ++k) c[k] = half2_less(c[k], (k & 2 ? y1 : y0) << (k & 1 ? 4 : 0));
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 const float p0 = x[n][0] * s0, p1 = x[n][1] * s0, p2 = x[n][2] * s1, p3 = x[n][3] * s1;
@@ -432,11 +431,6 @@ attend_kernel(const Args a) {
                 }
                 mma_f16(O[n][i][0], c[0], c[1], c[2], c[3], b0, b1);
                 mma_f16(O[n][i][1], c[4], c[5], c[6], c[7], b0, b1);
-                // (the zeros are taken off with the same rounded numbers, so that a value of zero adds exactly nothing)
-                const float z0 = zero_at(m0, i), z1 = zero_at(m1, i);
-                const float2 f0 = __half22float2(*(const __half2*)&h0), f1 = __half22float2(*(const __half2*)&h1);
-                zs[n][i][0] = fmaf(f0.x, z0, fmaf(f1.x, z1, zs[n][i][0]));
-                zs[n][i][1] = fmaf(f0.y, z0, fmaf(f1.y, z1, zs[n][i][1]));
             }
         }
         __syncwarp();
@@ -450,12 +444,7 @@ attend_kernel(const Args a) {
 #pragma unroll
         for (int o = 4; o < 32; o *= 2) {
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                sum[n][e] += __shfl_xor_sync(0xffffffffu, sum[n][e], o);
-                if (PARTS == 1)
-#pragma unroll
-                    for (int i = 0; i < NG; ++i) zs[n][i][e] += __shfl_xor_sync(0xffffffffu, zs[n][i][e], o);
-            }
+            for (int e = 0; e < 2; ++e) sum[n][e] += __shfl_xor_sync(0xffffffffu, sum[n][e], o);
             poison[n] |= __shfl_xor_sync(0xffffffffu, poison[n], o);
         }
         if (g == 0)
@@ -470,7 +459,7 @@ attend_kernel(const Args a) {
             for (int h = 0; h < 2; ++h)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    float2 v = make_float2(fmaf(O[n][i][h][e], PARTS == 2 ? 1.0f : 16777216.0f, -zs[n][i][e]), fmaf(O[n][i][h][2 + e], PARTS == 2 ? 0.0625f : 1048576.0f, -zs[n][i][e]));
+                    float2 v = make_float2(O[n][i][h][e] * 16777216.0f, O[n][i][h][2 + e] * 1048576.0f);
                     if (poison[n] >> (2 * i + e) & 1) v.x = v.y = __int_as_float(0x7fc00000);
                     *(float2*)(acc + (warp * COLS + n * 8 + 2 * t + e) * ROW + 32 * i + 4 * g + 2 * h) = v;
                 }
