@@ -10,14 +10,19 @@
 // its columns: nothing is wasted on padding up to eight heads. Scales and zeros are applied to what is small:
 //   score  Σ_groups s (Σ q' c − z Σ q'), q' = q times a power of two that brings a head's largest entry to 2^14 (exact for
 //          bfloat16; float32 as two float16 parts, 22 bits);
-//   output Σ_keys (p s) (c − z): p s is rounded to float16 (2^-11 of itself; float32: two parts, 2^-22) under a reference
-//          that holds it below 2^15, so that the scale s of a key's group of values costs no rounding of the values.
+//   output Σ_keys (p s) (c − z): p s as a float16 number (off by 2^-11 of itself; float32: two, the second times 2^11, 2^-22), so that
+//          the scale s of a key's group of values costs no rounding of the values.
 // The output's operands are c − z, differences of two such numbers, which are exact: tensor cores cut partial sums to 24 bits, and sums of
 // p s c are many times those of p s (c − z), which are nothing where the values are zeros. (With z Σ p s taken off at the end a value of
-// zero came to 2^-24 of 15 s a page. 64 sequences of 2,048 keys: 50.3 us so, 51.0 now; 40 tokens behind 6,000: 46.2 and 44.6.) With
-// float32 queries the scores' operands are c − z too, as 1024 + c less 1024 + z, and a page's sums are added in 32 bits.
-// The reference of a column follows its largest score, and the largest scale of the values, in steps: it moves only when a
-// score passes it by more than 2^8 or a scale passes the one it was made for; then the sums are multiplied by a power of two.
+// zero came to 2^-24 of 15 s a page.) With float32 queries the scores' operands are c − z too, as 1024 + c less 1024 + z, and a page's
+// sums are added in 32 bits.
+// Two references, both moved in powers of two. A column's scores have one that follows the largest in steps: it moves only when a score
+// passes it by more than 2^8. And p s is multiplied by a power of two of its own for EVERY column and group of 32 columns of the values,
+// lowered (with the group's sums) when a product would pass float16: its largest then lies in 2^8 .. 2^9, so that p s is off by no
+// less than 2^-33 of the group's largest (float32: 2^-44), whatever other groups, heads or keys of little weight hold. When the scores'
+// reference rises by a factor, these rise with it, and the sums stay as they are. (One reference for the largest scale of any group and key
+// lost whole groups behind one large value; it took 50.3 us at 64 sequences of 2,048 keys where this takes 51.8, 46.2 / 47.5 for 40 tokens
+// behind 6,000, 221 / 257 for 2,000 float32 tokens.)
 //
 // A page of a kv head is one run of bytes and arrives by one bulk copy in a ring; four warps take 16 of its keys each and keep
 // sums of their own, joined at the end in the order of the warps, then of the chunks: results do not depend on timing.
@@ -39,6 +44,7 @@ constexpr float LOG2E = 1.4426950408889634f;
 constexpr int WARPS = 4;
 constexpr int STAGES = 4;
 constexpr float STEP = 8.0f;                // how far a score may pass the reference, log2
+constexpr int MOST_NORM = 120;              // the largest power of two that p s is multiplied by, log2
 
 struct Args {
     const void* q;                 // [T][nh * hd]
@@ -129,10 +135,36 @@ __device__ __forceinline__ float zero_at(const uint32_t* m, int i) {
     return __uint_as_float(((i & 1 ? m[i >> 1] >> 16 : m[i >> 1]) & 15u) | 0x4b000000u) - 8388608.0f;
 }
 
+// powers of two
+__device__ __forceinline__ float two_to(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+__device__ __forceinline__ float log2_of(float v) { return (float)((int)(__float_as_uint(v) >> 23) - 127); }      // rounded down, v > 0
+// over a fragment's rows; what is not a number is left out
+__device__ __forceinline__ float column_max(float v) {
+    v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
+    v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
+    return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
+}
+// two at a time
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 r;
+    asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 r;
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\tfma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return r;
+}
+
 template <typename TQ, int NG, int NT>
 __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 2)
 attend_kernel(const Args a) {
     constexpr int HD = 32 * NG, PARTS = sizeof(TQ) == 4 ? 2 : 1, COLS = 8 * NT, TILE = kv4_tile_bytes(HD), MW = (NG + 1) / 2;
+    // groups of columns whose p s are formed before one vote whether they fit (64 sequences of 2,048 keys: 54.6 us with one, 52.3 with
+    // two, 53.1 with all four; float32, registers: 69.9 with one, 71.9 with two)
+    constexpr int AT_ONCE = PARTS == 2 ? 1 : 2;
     constexpr bool Q_HELD = NT == 1 && PARTS == 1;                   // the queries' operands in registers, else in shared memory
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES];
@@ -239,19 +271,21 @@ attend_kernel(const Args a) {
     }
     if (!Q_HELD) __syncthreads();
 
-    // top: the score (log2, rounded up) that a column's reference was made for; limit: how far a raw score may go under it
-    float O[NT][NG][2][4], sum[NT][2], ref[NT][2], top[NT][2], limit[NT][2];
+    // ref: the score (log2, rounded up) that a column's probabilities are relative to; limit: how far a raw score may go under it. O holds
+    // the sums times a power of two, norm, for every column and group of the values' columns
+    float O[NT][NG][2][4], norm[NT][NG][2], sum[NT][2], ref[NT][2], limit[NT][2];
     uint32_t poison[NT];
-    uint32_t s_bits = 0;                                             // the largest scale the references were made for, twice, zeros of 15
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         poison[n] = 0;
 #pragma unroll
-        for (int i = 0; i < NG; ++i)
+        for (int i = 0; i < NG; ++i) {
+            norm[n][i][0] = norm[n][i][1] = two_to(MOST_NORM);
 #pragma unroll
             for (int h = 0; h < 2; ++h) O[n][i][h][0] = O[n][i][h][1] = O[n][i][h][2] = O[n][i][h][3] = 0.0f;
+        }
 #pragma unroll
-        for (int e = 0; e < 2; ++e) { sum[n][e] = 0.0f; ref[n][e] = 0.0f; top[n][e] = limit[n][e] = -INFINITY; }
+        for (int e = 0; e < 2; ++e) { sum[n][e] = ref[n][e] = 0.0f; limit[n][e] = -INFINITY; }
     }
 
     for (int it = 0; it < n_pages; ++it) {
@@ -302,17 +336,15 @@ attend_kernel(const Args a) {
                     mma_f16(acc, c[4], c[5], c[6], c[7], qv.z, qv.w);
                 }
                 float (&y)[4] = x[n];
-                if (PARTS == 2) {
-                    y[0] = fmaf(s0, acc[0], y[0]);
-                    y[1] = fmaf(s0, acc[1], y[1]);
-                    y[2] = fmaf(s1, acc[2], y[2]);
-                    y[3] = fmaf(s1, acc[3], y[3]);
-                    continue;
+                float2 u = make_float2(acc[0], acc[1]), w = make_float2(acc[2], acc[3]);
+                if (PARTS == 1) {
+                    const float2 qq = make_float2(qs[n][i][0], qs[n][i][1]);
+                    u = fma2(make_float2(z0, z0), qq, u);
+                    w = fma2(make_float2(z1, z1), qq, w);
                 }
-                y[0] = fmaf(s0, fmaf(z0, qs[n][i][0], acc[0]), y[0]);
-                y[1] = fmaf(s0, fmaf(z0, qs[n][i][1], acc[1]), y[1]);
-                y[2] = fmaf(s1, fmaf(z1, qs[n][i][0], acc[2]), y[2]);
-                y[3] = fmaf(s1, fmaf(z1, qs[n][i][1], acc[3]), y[3]);
+                u = fma2(make_float2(s0, s0), u, make_float2(y[0], y[1]));
+                w = fma2(make_float2(s1, s1), w, make_float2(y[2], y[3]));
+                y[0] = u.x; y[1] = u.y; y[2] = w.x; y[3] = w.y;
             }
         }
         if (page_pos + KV4_PAGE - 1 > first_pos || (a.window && page_pos < last_pos + 1 - a.window)) {       // not all of it is seen by all
@@ -329,61 +361,32 @@ attend_kernel(const Args a) {
                 if (key + 8 > last_pos || key + 8 < lowest) m1[i] = 0;
             }
         }
-        // do the references hold?
-        uint32_t most = s_bits;
+        // does a score pass its column's reference by too much?
         bool moves = false;
-#pragma unroll
-        for (int i = 0; i < MW; ++i) most = __vmaxu2(most, __vmaxu2(m0[i], m1[i]));
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) moves |= x[n][e] > limit[n][e & 1];
-        if (__any_sync(0xffffffffu, moves || most != s_bits)) {
-            // scales that are not numbers: noted for the columns that see their keys, and taken as zero
-            most = 0;
+        if (__any_sync(0xffffffffu, moves)) {
 #pragma unroll
-            for (int i = 0; i < NG; ++i) {
-                const int sh = 16 * (i & 1);
-                const bool bad0 = ((m0[i >> 1] >> sh) & 0x7f80u) == 0x7f80u, bad1 = ((m1[i >> 1] >> sh) & 0x7f80u) == 0x7f80u;
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e)
-                        if ((bad0 && x[n][e] != -INFINITY) || (bad1 && x[n][2 + e] != -INFINITY)) poison[n] |= 1u << (2 * i + e);
-                if (bad0) m0[i >> 1] &= ~(0xffffu << sh);
-                if (bad1) m1[i >> 1] &= ~(0xffffu << sh);
-            }
-#pragma unroll
-            for (int i = 0; i < MW; ++i) most = __vmaxu2(most, __vmaxu2(m0[i], m1[i]));
-            most = max(most & 0xffffu, most >> 16) | 15u;             // (with every zero: what is compared is the whole half word)
-            s_bits = max(s_bits & 0xffffu, __reduce_max_sync(0xffffffffu, most)) * 0x10001u;
-            const float s_top = __uint_as_float((s_bits & 0xfff0u) << 16);
-            const float es = s_top > 0.0f ? (float)((int)(__float_as_uint(s_top) >> 23) - 126) : 0.0f;         // s_top < 2^es
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                float f[2];
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    float big = fmaxf(x[n][e], x[n][2 + e]);
-                    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 4));
-                    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 8));
-                    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 16));
-                    const bool had = top[n][e] != -INFINITY;
-                    if (big > limit[n][e]) {
-                        top[n][e] = ceilf(big * unit[n][e]);
-                        limit[n][e] = (top[n][e] + STEP) / unit[n][e];
+                    const float big = column_max(fmaxf(x[n][e], x[n][2 + e]));
+                    if (!(big > limit[n][e])) continue;
+                    const float top = ceilf(big * unit[n][e]), up = limit[n][e] != -INFINITY ? top - ref[n][e] : 0.0f;
+                    limit[n][e] = (top + STEP) / unit[n][e];
+                    ref[n][e] = top;
+                    sum[n][e] *= ex2(-up);
+                    // the sums of the values stay: their power of two rises by as much as the probabilities fall, as far as it goes
+#pragma unroll
+                    for (int i = 0; i < NG; ++i) {
+                        const float was = log2_of(norm[n][i][e]), now = fminf(was + up, MOST_NORM), f = ex2(now - was - up);
+                        norm[n][i][e] = two_to((int)now);
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) { O[n][i][h][e] *= f; O[n][i][h][2 + e] *= f; }
                     }
-                    const float was = ref[n][e];
-                    // p s <= 2^(STEP + top − ref + es) = 2^15; whole steps, so that the factors are powers of two
-                    ref[n][e] = top[n][e] != -INFINITY ? top[n][e] + es + STEP - 15.0f : 0.0f;
-                    f[e] = had ? ex2(was - ref[n][e]) : 1.0f;
-                    sum[n][e] *= f[e];
                 }
-#pragma unroll
-                for (int i = 0; i < NG; ++i)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) { O[n][i][h][0] *= f[0]; O[n][i][h][1] *= f[1]; O[n][i][h][2] *= f[0]; O[n][i][h][3] *= f[1]; }
-            }
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -401,36 +404,92 @@ attend_kernel(const Args a) {
             lds_halves<NG>(at + kv4_v_meta(HD) + p * (NG * 2), mz[k]);
         }
 #pragma unroll
-        for (int i = 0; i < NG; ++i) {
-            const float s0 = scale_at(m0, i), s1 = scale_at(m1, i);
-            const int half = i & 1 ? 0x7632 : 0x5410;
-            // keys t, 4 + t and 8 + t, 12 + t side by side
-            const uint32_t u0 = __byte_perm(v[0][i >> 1], v[1][i >> 1], half), u1 = __byte_perm(v[2][i >> 1], v[3][i >> 1], half);
-            const uint32_t w0 = u0 >> 8, w1 = u1 >> 8;
-            uint32_t c[8] = {u0 & 0x000f000fu, u0 & 0x00f000f0u, u1 & 0x000f000fu, u1 & 0x00f000f0u, w0 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x000f000fu, w1 & 0x00f000f0u};
-            const uint32_t y0 = __byte_perm(mz[0][i >> 1], mz[1][i >> 1], half) & 0x000f000fu, y1 = __byte_perm(mz[2][i >> 1], mz[3][i >> 1], half) & 0x000f000fu;
+        for (int i0 = 0; i0 < NG; i0 += AT_ONCE) {
+            // p s as float16 numbers
+            uint32_t h0[AT_ONCE][NT], h1[AT_ONCE][NT], over = 0;
+            auto weigh = [&](int i, int n, uint32_t& h0, uint32_t& h1, float s0, float s1) {
+                const float2 by = make_float2(norm[n][i][0], norm[n][i][1]);
+                const float2 p = mul2(mul2(make_float2(x[n][0], x[n][1]), make_float2(s0, s0)), by), w = mul2(mul2(make_float2(x[n][2], x[n][3]), make_float2(s1, s1)), by);
+                h0 = half2_of(p.x, p.y);
+                h1 = half2_of(w.x, w.y);
+            };
 #pragma unroll
-            for (int k = 0; k < 8; ++k) c[k] = half2_less(c[k], (k & 2 ? y1 : y0) << (k & 1 ? 4 : 0));
+            for (int i = i0; i < NG && i < i0 + AT_ONCE; ++i)
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                const float p0 = x[n][0] * s0, p1 = x[n][1] * s0, p2 = x[n][2] * s1, p3 = x[n][3] * s1;
-                const uint32_t h0 = half2_of(p0, p1), h1 = half2_of(p2, p3), b0 = transposed(h0), b1 = transposed(h1);
-                if (PARTS == 2) {
-                    // sums of a page of their own, added in 32 bits: the tensor cores' own additions cut instead of rounding
-                    const float2 f0 = __half22float2(*(const __half2*)&h0), f1 = __half22float2(*(const __half2*)&h1);
-                    const uint32_t l0 = transposed(half2_of(p0 - f0.x, p1 - f0.y)), l1 = transposed(half2_of(p2 - f1.x, p3 - f1.y));
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        float o[4] = {0.f, 0.f, 0.f, 0.f};
-                        mma_f16(o, c[4 * h], c[4 * h + 1], c[4 * h + 2], c[4 * h + 3], l0, l1);
-                        mma_f16(o, c[4 * h], c[4 * h + 1], c[4 * h + 2], c[4 * h + 3], b0, b1);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) O[n][i][h][e] += o[e];
-                    }
-                    continue;
+                for (int n = 0; n < NT; ++n) {
+                    weigh(i, n, h0[i - i0][n], h1[i - i0][n], scale_at(m0, i), scale_at(m1, i));
+                    over = __vimax3_u16x2(over, h0[i - i0][n], h1[i - i0][n]);
                 }
-                mma_f16(O[n][i][0], c[0], c[1], c[2], c[3], b0, b1);
-                mma_f16(O[n][i][1], c[4], c[5], c[6], c[7], b0, b1);
+            if (__any_sync(0xffffffffu, ((over + 0x04000400u) & 0x80008000u) != 0)) {        // beyond float16, or not a number
+#pragma unroll
+                for (int i = i0; i < NG && i < i0 + AT_ONCE; ++i) {
+                    // scales that are not numbers: noted for the columns that see their keys, and taken as zero
+                    float s0 = scale_at(m0, i), s1 = scale_at(m1, i);
+                    const bool bad0 = !(s0 < INFINITY), bad1 = !(s1 < INFINITY);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const int p = pos[n][e], from = a.window ? p - a.window : -1;
+                            if ((bad0 && key <= p && key > from) || (bad1 && key + 8 <= p && key + 8 > from)) poison[n] |= 1u << (2 * i + e);
+                        }
+                    if (bad0) { s0 = 0.0f; m0[i >> 1] &= i & 1 ? 0xffffu : 0xffff0000u; }
+                    if (bad1) { s1 = 0.0f; m1[i >> 1] &= i & 1 ? 0xffffu : 0xffff0000u; }
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const float big = column_max(fmaxf(x[n][e] * s0, x[n][2 + e] * s1));
+                            if (!(big * norm[n][i][e] > 32768.0f)) continue;
+                            const float now = two_to(8 - (int)log2_of(big)), f = ex2(log2_of(now) - log2_of(norm[n][i][e]));        // big · now in 2^8 .. 2^9
+                            norm[n][i][e] = now;
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) { O[n][i][h][e] *= f; O[n][i][h][2 + e] *= f; }
+                        }
+                        weigh(i, n, h0[i - i0][n], h1[i - i0][n], s0, s1);
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = i0; i < NG && i < i0 + AT_ONCE; ++i) {
+                const int half = i & 1 ? 0x7632 : 0x5410;
+                // keys t, 4 + t and 8 + t, 12 + t side by side
+                const uint32_t u0 = __byte_perm(v[0][i >> 1], v[1][i >> 1], half), u1 = __byte_perm(v[2][i >> 1], v[3][i >> 1], half);
+                const uint32_t w0 = u0 >> 8, w1 = u1 >> 8;
+                uint32_t c[8] = {u0 & 0x000f000fu, u0 & 0x00f000f0u, u1 & 0x000f000fu, u1 & 0x00f000f0u, w0 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x000f000fu, w1 & 0x00f000f0u};
+                const uint32_t y0 = __byte_perm(mz[0][i >> 1], mz[1][i >> 1], half) & 0x000f000fu, y1 = __byte_perm(mz[2][i >> 1], mz[3][i >> 1], half) & 0x000f000fu;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) c[k] = half2_less(c[k], (k & 2 ? y1 : y0) << (k & 1 ? 4 : 0));
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const uint32_t b0 = transposed(h0[i - i0][n]), b1 = transposed(h1[i - i0][n]);
+                    if (PARTS == 2) {
+                        // what is left of p s, times 2^11; sums of a page of their own, added in 32 bits: the tensor cores' own additions cut
+                        const float2 by = make_float2(norm[n][i][0], norm[n][i][1]);
+                        auto rest = [&](float p, float q, float s, uint32_t h) {
+                            const float2 f = __half22float2(*(const __half2*)&h), r = mul2(mul2(make_float2(p, q), make_float2(s, s)), by);
+                            const float2 d = mul2(fma2(f, make_float2(-1.0f, -1.0f), r), make_float2(2048.0f, 2048.0f));
+                            return transposed(half2_of(d.x, d.y));
+                        };
+                        const uint32_t l0 = rest(x[n][0], x[n][1], scale_at(m0, i), h0[i - i0][n]), l1 = rest(x[n][2], x[n][3], scale_at(m1, i), h1[i - i0][n]);
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            float o[4] = {0.f, 0.f, 0.f, 0.f}, l[4] = {0.f, 0.f, 0.f, 0.f};
+                            mma_f16(l, c[4 * h], c[4 * h + 1], c[4 * h + 2], c[4 * h + 3], l0, l1);
+                            mma_f16(o, c[4 * h], c[4 * h + 1], c[4 * h + 2], c[4 * h + 3], b0, b1);
+#pragma unroll
+                            for (int e = 0; e < 4; e += 2) {
+                                const float2 up = make_float2(4.8828125e-4f, 4.8828125e-4f), one = make_float2(1.0f, 1.0f);
+                                const float2 t = fma2(fma2(make_float2(l[e], l[e + 1]), up, make_float2(o[e], o[e + 1])), one, make_float2(O[n][i][h][e], O[n][i][h][e + 1]));
+                                O[n][i][h][e] = t.x;
+                                O[n][i][h][e + 1] = t.y;
+                            }
+                        }
+                        continue;
+                    }
+                    mma_f16(O[n][i][0], c[0], c[1], c[2], c[3], b0, b1);
+                    mma_f16(O[n][i][1], c[4], c[5], c[6], c[7], b0, b1);
+                }
             }
         }
         __syncwarp();
@@ -450,7 +509,7 @@ attend_kernel(const Args a) {
         if (g == 0)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                ref_s[warp][n * 8 + 2 * t + e] = top[n][e] == -INFINITY && sum[n][e] == 0.0f ? -INFINITY : ref[n][e];
+                ref_s[warp][n * 8 + 2 * t + e] = limit[n][e] == -INFINITY && sum[n][e] == 0.0f ? -INFINITY : ref[n][e];
                 sum_s[warp][n * 8 + 2 * t + e] = sum[n][e];
             }
 #pragma unroll
@@ -459,7 +518,8 @@ attend_kernel(const Args a) {
             for (int h = 0; h < 2; ++h)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    float2 v = make_float2(O[n][i][h][e] * 16777216.0f, O[n][i][h][2 + e] * 1048576.0f);
+                    const float back = __uint_as_float((254u << 23) - __float_as_uint(norm[n][i][e]));
+                    float2 v = make_float2(O[n][i][h][e] * (back * 16777216.0f), O[n][i][h][2 + e] * (back * 1048576.0f));
                     if (poison[n] >> (2 * i + e) & 1) v.x = v.y = __int_as_float(0x7fc00000);
                     *(float2*)(acc + (warp * COLS + n * 8 + 2 * t + e) * ROW + 32 * i + 4 * g + 2 * h) = v;
                 }
