@@ -591,10 +591,10 @@ join_kernel(const Args a, int hd) {
     float v[KV4_MAX_HD / 32] = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int c0 = 0; c0 < a.n_chunks; c0 += 32) {
         const float2 h = c0 + lane < a.n_chunks ? sp_ld_written(heads + c0 + lane) : make_float2(-INFINITY, 0.0f);
-        const float mine = h.x == -INFINITY ? 0.0f : ex2(h.x - big);
+        const float mine = h.x == -INFINITY ? -1.0f : ex2(h.x - big);
         for (int c = 0; c < min(32, a.n_chunks - c0); ++c) {
             const float w = __shfl_sync(0xffffffffu, mine, c);
-            if (w == 0.0f) continue;                                 // a chunk without a key that the row sees
+            if (w < 0.0f) continue;                                  // a chunk without a key that the row sees (one of weight zero counts where it is NaN)
 #pragma unroll
             for (int k = 0; k < KV4_MAX_HD / 32; ++k)
                 if (32 * k < hd) v[k] = fmaf(w, sp_ld_written(part + (size_t)(c0 + c) * hd + 32 * k + lane), v[k]);

@@ -108,3 +108,19 @@ def test_columns_of_zeros_stay_zeros(hd, dtype):
     for plan in (None, (1, 47, 1), (2, 10, 5)):
         out = attend(meta, pool, q, nh, nkv, hd, [1], None, None, plan)
         assert bool((out[0].cpu()[zero] == 0).all()) and bool((out[0].cpu()[~zero] != 0).all())
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_a_value_that_is_not_finite_counts_however_little_its_weight(dtype):
+    """Zero times NaN is NaN: a key of vanishing weight, in a chunk, a warp and a page of its own or among others."""
+    n, nh, nkv, hd = 400, 4, 2, 64
+    gen = torch.Generator().manual_seed(1)
+    q, k, v = (torch.randn(s, h, hd, generator=gen) for s, h in ((1, nh), (n, nkv), (n, nkv)))
+    q[..., 0], k[:, :, 0], k[0:64, :, 0] = 8.0, 0.0, -300.0          # the first page's scores are 300 below the others'
+    v[5, 0, 40] = float("inf")
+    q = q.to(dtype)
+    meta = KH.paged_meta([1], [n - 1], DEV)
+    pool = fill(meta, [(k, v)], nkv, hd)
+    for plan in (None, (1, 7, 1), (1, 1, 7), (2, 3, 3)):
+        out = attend(meta, pool, q, nh, nkv, hd, [1], None, None, plan).view(nh, hd).cpu()
+        assert bool(out[:2, 32:].isnan().all()) and bool(out[:2, :32].isfinite().all()) and bool(out[2:].isfinite().all()), plan
