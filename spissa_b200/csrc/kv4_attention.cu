@@ -177,8 +177,9 @@ attend_kernel(const Args a) {
     if (n_cols <= 0) return;
     const int first_pos = a.positions[tok0 + col0 / G], last_pos = a.positions[tok0 + (col0 + n_cols - 1) / G];        // of the tile's tokens
     const int lowest = a.window ? max(0, first_pos + 1 - a.window) : 0;
-    const int page0 = lowest / KV4_PAGE + chunk * a.chunk_pages, page1 = min(page0 + a.chunk_pages, last_pos / KV4_PAGE + 1);
-    const int n_pages = max(0, page1 - page0), row = sp_checked_row(a.seq_row[seq], a.rg);
+    // the last chunk takes what there is: a sequence may be longer than the split was made for
+    const int page0 = lowest / KV4_PAGE + chunk * a.chunk_pages, page_end = last_pos / KV4_PAGE + 1;
+    const int n_pages = max(0, (chunk + 1 == a.n_chunks ? page_end : min(page0 + a.chunk_pages, page_end)) - page0), row = sp_checked_row(a.seq_row[seq], a.rg);
     const int* table = a.page_table + (size_t)row * a.max_pages;
     constexpr int ROW = HD + 8;                                      // of the joined sums: neighbouring columns' rows lie in other banks
     float* acc = (float*)smem;                                       // [warp][column][ROW]

@@ -1991,7 +1991,8 @@ def kv4_attend_plan(n_seqs: int, nkv: int, hd: int, cols: int, pages: int) -> tu
 def kv4_attend(q, pool, out, meta, seq_start, n_seqs: int, max_new: int, longest: int, nh, nkv, hd, window, scale, sink=None, plan=None) -> None:
     """Attention of the step's tokens over the four-bit pages, every key read once per kv head and tile of query columns.
     ``seq_start`` [n_seqs + 1] int32, or None where every sequence brings one token; ``max_new``: the most tokens of a sequence;
-    ``longest``: the keys that the longest sequence may have (it shapes the split of the keys)."""
+    ``longest``: the keys that the longest sequence may have (it shapes the split of the keys; what a sequence has beyond goes to the last
+    chunk). ``plan``: the split, as ``kv4_attend_plan`` gives it."""
     T = q.shape[0]
     if q.dtype not in _DT or q.shape != (T, nh * hd) or out.shape != q.shape or out.dtype != q.dtype or nh % nkv:
         raise KernelError(f"kv4_attend: queries and output are [tokens, {nh} x {hd}] of one type, of heads in equal groups")
@@ -2004,6 +2005,8 @@ def kv4_attend(q, pool, out, meta, seq_start, n_seqs: int, max_new: int, longest
         raise KernelError(f"kv4_attend: at most {max_new} tokens of a sequence, {longest} keys of the longest")
     if seq_start is not None and (seq_start.dtype != torch.int32 or seq_start.numel() < n_seqs + 1):
         raise KernelError("kv4_attend: the sequences' first tokens are int32, one more than sequences")
+    if meta.seq_slot.numel() < n_seqs:
+        raise KernelError(f"kv4_attend: a row of the page table for each of {n_seqs} sequences is wanted, got {meta.seq_slot.numel()}")
     lib = load("kv4_attention")
     pt = meta.page_table
     window = int(window or 0)
@@ -2011,6 +2014,8 @@ def kv4_attend(q, pool, out, meta, seq_start, n_seqs: int, max_new: int, longest
     if window:
         pages = min(pages, (window + max_new - 2) // 64 + 2)
     nt, chunk_pages, n_chunks = plan or kv4_attend_plan(n_seqs, nkv, hd, max_new * (nh // nkv), max(1, pages))
+    if chunk_pages * n_chunks < pages:
+        raise KernelError(f"kv4_attend: {n_chunks} chunks of {chunk_pages} pages do not hold the {pages} of {longest} keys")
     need = T * nh * n_chunks * (hd + 2) if n_chunks > 1 else 0
     scratch = torch.empty(need, dtype=torch.float32, device=q.device) if need else None
     if _RANGE_CHECKED["kv4_attention"]:

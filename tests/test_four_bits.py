@@ -121,3 +121,11 @@ def test_the_plain_statement_of_the_format():
     reach = x.double().amax(1).clamp(min=0) - x.double().amin(1).clamp(max=0)
     # z is rounded too, so an end of the range may be cut by half a step on top of the half step of its code
     assert bool(((y - x.double()).abs().amax(1) <= reach / 15 * 9 / 8).all())
+
+
+def test_a_split_of_the_keys_covers_them():
+    from spissa_b200.csrc.lib import kv4_attend_plan
+    for n_seqs, nkv, hd, cols in ((1, 8, 64, 4), (64, 8, 128, 4), (3, 8, 128, 4), (1, 8, 128, 160), (200, 2, 96, 3), (5, 1, 32, 33)):
+        for pages in (1, 2, 5, 33, 64, 641, 2000):
+            nt, each, n = kv4_attend_plan(n_seqs, nkv, hd, cols, pages)
+            assert nt in (1, 2) and n >= 1 and each * n >= pages > each * (n - 1)

@@ -124,3 +124,44 @@ def test_a_value_that_is_not_finite_counts_however_little_its_weight(dtype):
     for plan in (None, (1, 7, 1), (1, 1, 7), (2, 3, 3)):
         out = attend(meta, pool, q, nh, nkv, hd, [1], None, None, plan).view(nh, hd).cpu()
         assert bool(out[:2, 32:].isnan().all()) and bool(out[:2, :32].isfinite().all()) and bool(out[2:].isfinite().all()), plan
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_a_sequence_longer_than_its_split_keeps_its_newest_keys(dtype):
+    """``longest`` shapes the split; a sequence that has more keys than it says is read to its end."""
+    from spissa_b200.csrc import lib
+    n, nh, nkv, hd = 700, 4, 2, 64
+    gen = torch.Generator().manual_seed(2)
+    q, k, v = (torch.randn(s, h, hd, generator=gen) for s, h in ((1, nh), (n, nkv), (n, nkv)))
+    q = q.to(dtype)
+    want, tol = expected(q, [(k, v)], [1], [n - 1], 1.0 / math.sqrt(hd))
+    meta = KH.paged_meta([1], [n - 1], DEV)
+    pool, rows = fill(meta, [(k, v)], nkv, hd), q.to(DEV).reshape(1, -1)
+    for longest in (1, 64, 300, 699):
+        for window in (None, 650):
+            out = torch.empty_like(rows)
+            lib.kv4_attend(rows, pool, out, meta, None, 1, 1, longest, nh, nkv, hd, window, 1.0 / math.sqrt(hd))
+            if window is None:
+                holds(out, want, tol, longest)
+            else:
+                holds(out, *expected(q, [(k, v)], [1], [n - 1], 1.0 / math.sqrt(hd), window), (longest, window))
+
+
+def test_what_a_split_and_the_rows_of_the_table_have_to_cover():
+    from types import SimpleNamespace
+
+    from spissa_b200.csrc import lib
+    nh, nkv, hd = 4, 2, 64
+    meta = KH.paged_meta([1, 1], [300, 20], DEV)
+    pool, q = lib.kv4_pool(meta.n_pages, nkv, hd, DEV), torch.zeros(2, nh * hd, dtype=BF, device=DEV)
+
+    def call(meta=meta, window=None, plan=None):
+        lib.kv4_attend(q, pool, torch.empty_like(q), meta, None, 2, 1, 301, nh, nkv, hd, window, 0.125, None, plan)
+    for plan in (None, (1, 5, 1), (2, 1, 5), (1, 2, 3)):
+        call(plan=plan)
+    call(window=60, plan=(1, 1, 2))
+    for bad in (lambda: call(plan=(1, 4, 1)), lambda: call(plan=(1, 1, 4)), lambda: call(plan=(2, 2, 2)), lambda: call(window=60, plan=(1, 1, 1)),
+                lambda: call(meta=SimpleNamespace(**{**vars(meta), "seq_slot": meta.seq_slot[:1]}))):
+        with pytest.raises(lib.KernelError):
+            bad()
+    lib.check_status(DEV)
