@@ -295,10 +295,10 @@ attend_kernel(const Args a) {
             const int i = it - 1 + STAGES;
             if (i % 32 == 0) hold(i);
             const int page = __shfl_sync(0xffffffffu, held, i % 32);
-            if (lane == 0 && mbar_wait_flag(smem_u32(&empty[(it - 1) % STAGES]), ((it - 1) / STAGES) & 1, a.status, 141, &failed)) fetch(i, page);
+            if (lane == 0 && mbar_wait_flag(smem_u32(&empty[(it - 1) % STAGES]), ((it - 1) / STAGES) & 1, a.status, 171, &failed)) fetch(i, page);
         }
         __syncwarp();
-        mbar_wait_flag(smem_u32(&full[it % STAGES]), (it / STAGES) & 1, a.status, 142, &failed);
+        mbar_wait_flag(smem_u32(&full[it % STAGES]), (it / STAGES) & 1, a.status, 172, &failed);
         const int page_pos = (page0 + it) * KV4_PAGE;
         const uint32_t at = ring + (it % STAGES) * TILE;
         const int r0 = warp * 16 + g;                            // rows of the page's keys as they lie: this lane's are r0 and r0 + 8

@@ -499,15 +499,22 @@ STATUS_TEXT = {101: "the TMA loader waited too long for a free pipeline stage",
                115: "attention: the softmax warps waited too long for the scores",
                116: "attention: the softmax warps waited too long for the previous block's output",
                117: "attention: the softmax warps waited too long for the last block's output",
-               141: "rglru: the MMA issuer waited too long for the gate matrices",
-               142: "rglru: the convolution warps waited too long for their buffer",
-               143: "rglru: the MMA issuer waited too long for a free accumulator",
-               144: "rglru: the MMA issuer waited too long for the convolution",
-               145: "rglru: the recurrence warps waited too long for the gates",
+               161: "rglru: the MMA issuer waited too long for the gate matrices",
+               162: "rglru: the convolution warps waited too long for their buffer",
+               163: "rglru: the MMA issuer waited too long for a free accumulator",
+               164: "rglru: the MMA issuer waited too long for the convolution",
+               165: "rglru: the recurrence warps waited too long for the gates",
                151: "mlstm: the chunks' sums waited too long for their products",
                152: "mlstm: a stage of the outputs' operands did not become free in time",
                153: "mlstm: the products with the start states took too long",
                154: "mlstm: the products with the values took too long",
+               171: "kv4_attention: the loader waited too long for a free page of the ring",
+               172: "kv4_attention: a warp waited too long for a page",
+               181: "q4_tc: the loader waited too long for a free stage",
+               182: "q4_tc: the MMA issuer waited too long for the codes' numbers",
+               183: "q4_tc: the working warps waited too long for a stage",
+               184: "q4_tc: the working warps waited too long for the accumulator",
+               185: "q4_tc: the working warps waited too long for tensor memory to become free",
                301: "embedding: a token id outside the vocabulary",
                401: "range check: a page index from a page table lies beyond the pools",
                402: "range check: a sequence's row lies beyond the page table",

@@ -131,7 +131,7 @@ q4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ 
             int s = 0;
             uint32_t ph = 1;
             for (int b = b0; b < b1; ++b) {
-                if (!wait_for(smem_u32(&bar_empty[s]), ph, a.status, 151, &failed)) break;
+                if (!wait_for(smem_u32(&bar_empty[s]), ph, a.status, 181, &failed)) break;
                 const uint32_t to = base + (uint32_t)s * stage_bytes, bar = smem_u32(&bar_full[s]);
                 mbar_expect_tx(bar, stage_bytes_in);
                 tma_load_4d(to + x_bytes, &map_codes, 0, 0, b, row_tile * TILES, bar);
@@ -147,7 +147,7 @@ q4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ 
             int s = 0, slot = 0;
             uint32_t slot_ph = 0;
             for (int b = b0; b < b1; ++b) {
-                if (!wait_for(smem_u32(&bar_a[slot]), slot_ph, a.status, 153, &failed)) break;
+                if (!wait_for(smem_u32(&bar_a[slot]), slot_ph, a.status, 182, &failed)) break;
                 tc_fence_after();                                    // (x is there too: those who took the codes apart have waited for it)
                 const uint32_t x_at = base + (uint32_t)s * stage_bytes, a_at = tmem + a.d_cols + slot * A_COLS;
 #pragma unroll
@@ -175,8 +175,8 @@ q4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ 
         int s = turn, slot = turn;
         uint32_t ph = 0, slot_ph = 1;
         for (int b = b0 + turn; b < b1; b += 2) {
-            if (!wait_for(smem_u32(&bar_used[slot]), slot_ph, a.status, 156, &failed)) break;            // what the slot held has been multiplied
-            if (!wait_for(smem_u32(&bar_full[s]), ph, a.status, 154, &failed)) break;
+            if (!wait_for(smem_u32(&bar_used[slot]), slot_ph, a.status, 185, &failed)) break;            // what the slot held has been multiplied
+            if (!wait_for(smem_u32(&bar_full[s]), ph, a.status, 183, &failed)) break;
             tc_fence_after();
             const uint32_t at = base + (uint32_t)s * stage_bytes + x_bytes, codes = at + tile * 1024 + hi * 8;
             const uint32_t meta = at + TILES * 1024 + tile * q4w_meta_bytes(GROUP) + g * (512 / GROUP) + hi * 2;
@@ -205,7 +205,7 @@ q4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ 
             if ((s += 2) >= a.stages) { s -= a.stages; ph ^= 1u; }
             if ((slot += 2) >= a.slots) { slot = turn; slot_ph ^= 1u; }
         }
-        wait_for(smem_u32(&bar_acc), 0, a.status, 155, &failed);
+        wait_for(smem_u32(&bar_acc), 0, a.status, 184, &failed);
         tc_fence_after();
         // the accumulator into shared memory (the stages are free by now), [row of x][128 rows of W]
         asm volatile("bar.sync 1, 512;" ::: "memory");

@@ -487,15 +487,15 @@ rglru_chunk_tc_kernel(const __grid_constant__ CUtensorMap map_r, const __grid_co
     if (warp == 1) {
         if (lane == 0) {
             constexpr uint32_t idesc = umma_idesc_bf16(RT_ROWS, 2 * RT_CHUNK);
-            bool ok = mbar_wait(smem_u32(&bar_w), 0, status, 141);
+            bool ok = mbar_wait(smem_u32(&bar_w), 0, status, 161);
             uint32_t it = 0;
             RgPlace pl;
             RgWalk walk;
             for (int x = walker; x < n_chunks && ok; x += walkers) {
                 if (!walk.place(a, RT_CHUNK, x, pl)) continue;
                 const uint32_t buf = it & 1u, phase = (it >> 1) & 1u;
-                ok = mbar_wait(smem_u32(&bar_acc_free[buf]), phase ^ 1u, status, 143) &&
-                     mbar_wait(smem_u32(&bar_u_full[buf]), phase, status, 144);
+                ok = mbar_wait(smem_u32(&bar_acc_free[buf]), phase ^ 1u, status, 163) &&
+                     mbar_wait(smem_u32(&bar_u_full[buf]), phase, status, 164);
                 if (!ok) break;
                 tc_fence_after();
 #pragma unroll
@@ -538,7 +538,7 @@ rglru_chunk_tc_kernel(const __grid_constant__ CUtensorMap map_r, const __grid_co
             if ((!last_j || more) && row0 < np.n) nxt.fetch(a, np, np.t0 + row0, np.t0 + np.n, c + nj * 64);
             const uint32_t buf = it & 1u;
             if (j == 0) {
-                ok = mbar_wait(smem_u32(&bar_u_free[buf]), ((it >> 1) & 1u) ^ 1u, status, 142);
+                ok = mbar_wait(smem_u32(&bar_u_free[buf]), ((it >> 1) & 1u) ^ 1u, status, 162);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
             }
@@ -587,7 +587,7 @@ rglru_chunk_tc_kernel(const __grid_constant__ CUtensorMap map_r, const __grid_co
             const uint32_t phase = (it >> 1) & 1u;
             ++it;
             // (the convolution's own barrier too: this warp reads what those warps stored)
-            ok = mbar_wait(smem_u32(&bar_u_full[group]), phase, status, 145) && mbar_wait(smem_u32(&bar_acc[group]), phase, status, 145);
+            ok = mbar_wait(smem_u32(&bar_u_full[group]), phase, status, 165) && mbar_wait(smem_u32(&bar_acc[group]), phase, status, 165);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             tc_fence_after();
