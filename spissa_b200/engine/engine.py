@@ -131,8 +131,9 @@ class Engine:
         dev = _require_gpu(device)
         config = load_config(folder)
         model = Model(config.to_spec())
-        model.check_bits(weight_bits, cache_bits)                         # before a large file is read
-        kernel_build.prefetch(model.kernel_modules(_DTYPES[dtype]))       # in the background, while the weights are read
+        rt = Runtime(dev, _DTYPES[dtype], cls.PAGE_SIZE, int(weight_bits), int(cache_bits))
+        model.check_bits(rt.weight_bits, rt.cache_bits)                   # before a large file is read
+        kernel_build.prefetch(model.kernel_modules(rt.act_dtype, rt))     # in the background, while the weights are read
         tensors = load_tensors(folder, model.weight_specs(), dev, _DTYPES[dtype] == torch.float32)
         return cls(config, tensors, dtype, max_tokens, max_seqs, device, use_graphs, fuse_decode, fuse_prefill, weight_bits, cache_bits)
 

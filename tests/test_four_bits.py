@@ -129,3 +129,22 @@ def test_a_split_of_the_keys_covers_them():
         for pages in (1, 2, 5, 33, 64, 641, 2000):
             nt, each, n = kv4_attend_plan(n_seqs, nkv, hd, cols, pages)
             assert nt in (1, 2) and n >= 1 and each * n >= pages > each * (n - 1)
+
+
+@pytest.mark.parametrize("weight_bits,cache_bits,more", [(16, 16, set()), (4, 16, {"q4", "q4_tc"}), (16, 4, {"kv4", "kv4_attention"}),
+                                                         (4, 4, {"q4", "q4_tc", "kv4", "kv4_attention"})])
+def test_the_libraries_are_asked_for_before_the_weights_are_read(weight_bits, cache_bits, more, monkeypatch, tmp_path):
+    import json
+
+    from spissa_b200.engine import engine as E
+    (tmp_path / "config.json").write_text(json.dumps(TINY_E))
+    asked = []
+    monkeypatch.setattr(E, "_require_gpu", lambda device: torch.device("cpu"))
+    monkeypatch.setattr(E.kernel_build, "prefetch", lambda names: asked.append(set(names)))
+
+    def read(*args):
+        raise InterruptedError
+    monkeypatch.setattr(E, "load_tensors", read)
+    with pytest.raises(InterruptedError):
+        E.Engine.from_folder(tmp_path, weight_bits=weight_bits, cache_bits=cache_bits)
+    assert len(asked) == 1 and asked[0] & {"q4", "q4_tc", "kv4", "kv4_attention"} == more and "generic" in asked[0]
