@@ -1973,18 +1973,22 @@ def kv4_unpack_pages(pool, meta, k_out, v_out, table, step, window, nkv, hd) -> 
         c_void_p(_stream())))
 
 
+def kv4_room(hd: int) -> int:
+    """Tiles of sixteen query columns that ``kv4_attend`` runs at once: two CTAs of an SM, three of heads up to 64."""
+    return 296 if hd > 64 else 444
+
+
 @functools.lru_cache(maxsize=4096)
 def kv4_attend_plan(n_seqs: int, nkv: int, hd: int, cols: int, pages: int) -> tuple:
     """(tiles of eight columns a CTA takes, pages per chunk, chunks) for ``kv4_attend``: ``cols`` query columns (heads of a kv head
     times tokens) of the sequence with the most, ``pages`` of keys that the longest sequence's tokens see.
 
-    By rounds of the CTAs that find room (four of an SM with eight columns, two with sixteen, three of heads up to 64) times what one takes:
-    its pages and about three more for setting up and joining its warps' sums; the chunks' joining costs two and a third of one per chunk. Measured (us, as
-    chosen / otherwise): 64 sequences of 2,048 keys 50 in one chunk, 52 in two, 56 in four; 3 of about 50,000 71 in 24, 77 in 16, 81 in
-    32; one of 2,048 10.7 in eleven, 10.3 in seven, 12.3 in seventeen; 40 tokens behind 6,000 46 in three, 52 in six; with
-    heads of 64 31 in five, 36 in three."""
+    By rounds of the CTAs that find room (four of an SM with eight columns, ``kv4_room`` with sixteen) times what one takes: its pages and
+    about three more for setting up and joining its warps' sums; the chunks' joining costs two and a third of one per chunk. Measured (us,
+    as chosen / otherwise): 64 sequences of 2,048 keys 53 in one chunk, 57 in two, 61 in four; 3 of about 50,000 75 in 24, 82 in 16, 87 in
+    32; one of 2,048 10.8 in ten, 10.7 in eight, 11.3 in fourteen; 40 tokens behind 6,000 48 in three, 55 in six."""
     nt = 1 if cols <= 8 else 2
-    base, room = n_seqs * nkv * -(-cols // (8 * nt)), 592 if nt == 1 else 296 if hd > 64 else 444
+    base, room = n_seqs * nkv * -(-cols // (8 * nt)), 592 if nt == 1 else kv4_room(hd)
     best = None
     for n in range(1, min(pages, max(1, 2 * room // base)) + 1):
         each = -(-pages // n)

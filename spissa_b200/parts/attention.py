@@ -225,15 +225,19 @@ def attend_paged(q, step, cache, nh, nkv, hd, window, scale, sink=None, counters
     return ctx
 
 
-def reads_codes(q, cols: int, nkv: int) -> bool:
+def reads_codes(q, cols: int, nkv: int, hd: int = 128, n_seqs: int = 1) -> bool:
     """Whether a prompt step's attention works on the codes of a four-bit cache, or on its pages unpacked first. ``cols``: the most
-    query columns of a sequence. On the codes every 16 columns take a page apart again; unpacked, short steps meet the tile
-    kernels, which take a sequence's keys one after another. Measured, us (codes / unpacked first), 32 heads on 8 of 128:
-      bfloat16, tokens behind 2,000: 64 32/75, 192 80/81, 256 94/59, 1,024 358/78; 1,024 tokens of 64 sequences behind 1,000 172/286;
-      float32, tokens behind nothing: 64 10/28, 512 58/148, 2,000 434/1,490; 512 behind 2,000 243/961."""
+    query columns of a sequence. On the codes every 16 columns take a page apart again; unpacked, steps meet the tile kernels, which take
+    a sequence's keys one after another, in a time that hardly depends on the tokens while all tiles run at once. So the codes win while
+    THEIR tiles find room on the SMs at once (``lib.kv4_room``). Measured, us (codes / unpacked first), bfloat16, one sequence:
+      32 heads on 8 of 128, behind 2,000: 64 tokens 32/75, 128 50/76, 192 81/78, 256 95/58, 1,024 365/75; behind 100,000: 128 1,748/3,102, 256 3,478/2,364;
+      32 on 8 of 64, behind 2,000: 192 41/47, 256 65/36;    32 on 8 of 96: 192 77/57, 512 161/62;    32 on 8 of 32: 192 31/33, 512 66/44;
+      9 on 3 of 96, behind 2,000: 256 29/55, 512 46/60, 1,024 96/69; behind 100,000: 256 748/2,316;    12 on 12 of 96: 384 45/61, 512 82/64;
+      16 on 1 of 128, behind 2,000: 256 50/53, 512 100/57;    6 on 2 of 32: 512 24/36, 1,024 40/42; behind 100,000: 512 548/1,129;
+    1,024 tokens of 64 sequences behind 1,000 (32 on 8 of 128): 180/283; float32: 512 tokens behind nothing 66/146, behind 2,000 256/960."""
     if q.dtype == torch.float32:
         return nkv * -(-cols // 16) < 1 << 16            # (tiles of columns are a grid's second dimension)
-    return q.shape[0] < FLASH_TC_TOKENS or cols <= SPLIT4_COLUMNS
+    return q.shape[0] < FLASH_TC_TOKENS or cols <= SPLIT4_COLUMNS or n_seqs * nkv * -(-cols // 16) <= K.kv4_room(hd)
 
 
 def attend_four_bits(q, step, cache, nh, nkv, hd, window, scale, sink=None):
@@ -243,7 +247,7 @@ def attend_four_bits(q, step, cache, nh, nkv, hd, window, scale, sink=None):
         raise K.KernelError(f"attention: queries are [tokens, {nh} x {hd}], bfloat16 or float32, of heads in equal groups")
     if not scale > 0:
         raise K.KernelError(f"attention over a four-bit cache takes a positive scale, got {scale}")
-    if step.all_single or reads_codes(q, step.max_new * (nh // nkv), nkv):
+    if step.all_single or reads_codes(q, step.max_new * (nh // nkv), nkv, hd, step.n_seqs):
         out = torch.empty_like(q)
         # (a decode step by its length's bucket, as below: run directly and replayed from a graph it adds up in the same order)
         longest = length_bucket(step.max_len, cache.page_size) if step.all_single else step.max_len

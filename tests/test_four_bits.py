@@ -148,3 +148,18 @@ def test_the_libraries_are_asked_for_before_the_weights_are_read(weight_bits, ca
     with pytest.raises(InterruptedError):
         E.Engine.from_folder(tmp_path, weight_bits=weight_bits, cache_bits=cache_bits)
     assert len(asked) == 1 and asked[0] & {"q4", "q4_tc", "kv4", "kv4_attention"} == more and "generic" in asked[0]
+
+
+def test_which_prompt_steps_read_the_codes():
+    """Those whose tiles of sixteen query columns find room at once, whatever the head's size; and short ones."""
+    from spissa_b200.csrc.lib import kv4_room
+    from spissa_b200.parts.attention import reads_codes
+
+    def takes(T, n_seqs, max_new, nh, nkv, hd):
+        return reads_codes(torch.empty(T, 1, dtype=torch.bfloat16), max_new * (nh // nkv), nkv, hd, n_seqs)
+    assert kv4_room(32) == kv4_room(64) > kv4_room(96) == kv4_room(128)
+    for T, nh, nkv, hd, want in ((255, 32, 8, 128, True), (256, 32, 8, 128, False), (256, 16, 1, 128, True), (512, 16, 1, 128, False),
+                                 (512, 9, 3, 96, True), (1024, 9, 3, 96, False), (384, 12, 12, 96, True), (512, 12, 12, 96, False),
+                                 (1024, 6, 2, 32, True), (384, 16, 4, 32, True), (512, 16, 4, 32, False), (256, 32, 8, 64, False)):
+        assert takes(T, 1, T, nh, nkv, hd) is want, (T, nh, nkv, hd)
+    assert takes(1024, 64, 24, 32, 8, 128) and not takes(2048, 16, 128, 32, 8, 128) and not takes(2000, 3, 900, 32, 8, 128)
