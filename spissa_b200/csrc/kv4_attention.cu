@@ -8,14 +8,14 @@
 // four bits in the lowest place of a half word ARE the float16 c · 2^-24, one place up 16 c · 2^-24, so an AND makes an operand
 // of mma.sync m16n8k16, with 16 keys (scores) or 16 columns of the values (output) as its rows and the query columns as
 // its columns: nothing is wasted on padding up to eight heads. Scales and zeros are applied to what is small:
-//   score  Σ_groups s (Σ q' c − z Σ q'), q' = q times a power of two that brings a head's largest entry to 2^14 (exact for
-//          bfloat16; float32 as two float16 parts, 22 bits);
+//   score  Σ_groups s Σ q' (c − z), q' = q times a power of two that brings a head's largest entry to 2^14: exact for bfloat16 entries
+//          down to 2^-27 of the largest, off by 2^-35 of the largest below; float32 as two such numbers, 22 bits;
 //   output Σ_keys (p s) (c − z): p s as a float16 number (off by 2^-11 of itself; float32: two, the second times 2^11, 2^-22), so that
 //          the scale s of a key's group of values costs no rounding of the values.
-// The output's operands are c − z, differences of two such numbers, which are exact: tensor cores cut partial sums to 24 bits, and sums of
-// p s c are many times those of p s (c − z), which are nothing where the values are zeros. (With z Σ p s taken off at the end a value of
-// zero came to 2^-24 of 15 s a page.) With float32 queries the scores' operands are c − z too, as 1024 + c less 1024 + z, and a page's
-// sums are added in 32 bits.
+// The operands are c − z, differences of two such numbers, which are exact: tensor cores cut partial sums to 24 bits, and sums of codes are
+// many times those of c − z, which are nothing where keys or values are zeros beside a large one of their group. (With z Σ q' and z Σ p s
+// taken off at the end a value of zero came to 2^-24 of 15 s a page, and a column's largest key to errors of the scores; the time is the
+// same.) With float32 queries a page's sums are added in 32 bits.
 // Two references, both moved in powers of two. A column's scores have one that follows the largest in steps: it moves only when a score
 // passes it by more than 2^8. And p s is multiplied by a power of two of its own for EVERY column and group of 32 columns of the values,
 // lowered (with the group's sums) when a product would pass float16: its largest then lies in 2^8 .. 2^9, so that p s is off by no
@@ -81,11 +81,6 @@ __device__ __forceinline__ uint32_t half2_of(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *(const uint32_t*)&h;
 }
-// of two pairs of float16 numbers, subnormal ones as any other
-__device__ __forceinline__ uint32_t half2_less(uint32_t a, uint32_t b) {
-    const __half2 r = __hsub2(*(const __half2*)&a, *(const __half2*)&b);
-    return *(const uint32_t*)&r;
-}
 __device__ __forceinline__ uint4 lds16(uint32_t at) {
     uint4 v;
     asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
@@ -131,10 +126,6 @@ __device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
 __device__ __forceinline__ float scale_at(const uint32_t* m, int i) {
     return __uint_as_float(i & 1 ? m[i >> 1] & 0xfff00000u : (m[i >> 1] << 16) & 0xfff00000u);
 }
-__device__ __forceinline__ float zero_at(const uint32_t* m, int i) {
-    return __uint_as_float(((i & 1 ? m[i >> 1] >> 16 : m[i >> 1]) & 15u) | 0x4b000000u) - 8388608.0f;
-}
-
 // powers of two
 __device__ __forceinline__ float two_to(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 __device__ __forceinline__ float log2_of(float v) { return (float)((int)(__float_as_uint(v) >> 23) - 127); }      // rounded down, v > 0
@@ -214,7 +205,7 @@ attend_kernel(const Args a) {
 
     // The queries: lane (column g, dims 32 i + 8 t ..). Columns that are not there are zeros and see nothing.
     uint32_t qh[Q_HELD ? NG : 1][4];
-    float unit[NT][2], qs[NT][NG][2];                                // of columns 2 t and 2 t + 1
+    float unit[NT][2];                                               // of columns 2 t and 2 t + 1
     int pos[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -234,26 +225,19 @@ attend_kernel(const Args a) {
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         const int up = top > 0.0f ? min(94, max(-94, 141 - (int)(__float_as_uint(top) >> 23))) : 0;
-        const float by = __uint_as_float((uint32_t)(127 + up) << 23), back = __uint_as_float((uint32_t)((PARTS == 2 ? 127 : 151) - up) << 23) * a.scale * LOG2E;
+        const float by = __uint_as_float((uint32_t)(127 + up) << 23), back = __uint_as_float((uint32_t)(151 - up) << 23) * a.scale * LOG2E;
 #pragma unroll
         for (int i = 0; i < NG; ++i) {
-            float sum = 0.0f;
             uint32_t h[PARTS][4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const float lo = v[i][2 * j] * by, hi = v[i][2 * j + 1] * by, f = j & 1 ? 0.0625f : 1.0f;
-                sum += lo + hi;
                 h[0][j] = half2_of(lo * f, hi * f);
                 if (PARTS == 2) {
                     const float2 first = __half22float2(*(const __half2*)&h[0][j]);
                     h[PARTS - 1][j] = half2_of(lo * f - first.x, hi * f - first.y);
                 }
             }
-            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-            sum *= -5.9604644775390625e-8f;                          // −2^-24 Σ q', in the units of the codes' products
-            qs[n][i][0] = __shfl_sync(0xffffffffu, sum, 8 * t);
-            qs[n][i][1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4);
             if (Q_HELD) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) qh[Q_HELD ? i : 0][j] = h[0][j];
@@ -317,14 +301,12 @@ attend_kernel(const Args a) {
         lds_halves<NG>(at + kv4_v_meta(HD) + (p0 + 8) * (NG * 2), m1);
 #pragma unroll
         for (int i = 0; i < NG; ++i) {
-            const float s0 = scale_at(km0, i), s1 = scale_at(km1, i), z0 = zero_at(km0, i), z1 = zero_at(km1, i);
+            const float s0 = scale_at(km0, i), s1 = scale_at(km1, i);
             const uint32_t u0 = k0[i], u1 = k1[i], w0 = u0 >> 8, w1 = u1 >> 8;
             uint32_t c[8] = {u0 & 0x000f000fu, u1 & 0x000f000fu, u0 & 0x00f000f0u, u1 & 0x00f000f0u, w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u};
-            if (PARTS == 2) {
-                const uint32_t y0 = ((km0[i >> 1] >> (16 * (i & 1))) & 15u) * 0x10001u, y1 = ((km1[i >> 1] >> (16 * (i & 1))) & 15u) * 0x10001u;
+            const uint32_t y0 = __byte_perm(km0[i >> 1], 0, i & 1 ? 0x3232 : 0x1010) & 0x000f000fu, y1 = __byte_perm(km1[i >> 1], 0, i & 1 ? 0x3232 : 0x1010) & 0x000f000fu;
 #pragma unroll
-                for (int k = 0; k < 8; ++k) c[k] = q4_less(c[k], (k & 1 ? y1 : y0) << (k & 2 ? 4 : 0));
-            }
+            for (int k = 0; k < 8; ++k) c[k] = q4_minus(c[k], (k & 1 ? y1 : y0) << (k & 2 ? 4 : 0));
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 float acc[4] = {0.f, 0.f, 0.f, 0.f};
@@ -337,14 +319,8 @@ attend_kernel(const Args a) {
                     mma_f16(acc, c[4], c[5], c[6], c[7], qv.z, qv.w);
                 }
                 float (&y)[4] = x[n];
-                float2 u = make_float2(acc[0], acc[1]), w = make_float2(acc[2], acc[3]);
-                if (PARTS == 1) {
-                    const float2 qq = make_float2(qs[n][i][0], qs[n][i][1]);
-                    u = fma2(make_float2(z0, z0), qq, u);
-                    w = fma2(make_float2(z1, z1), qq, w);
-                }
-                u = fma2(make_float2(s0, s0), u, make_float2(y[0], y[1]));
-                w = fma2(make_float2(s1, s1), w, make_float2(y[2], y[3]));
+                const float2 u = fma2(make_float2(s0, s0), make_float2(acc[0], acc[1]), make_float2(y[0], y[1]));
+                const float2 w = fma2(make_float2(s1, s1), make_float2(acc[2], acc[3]), make_float2(y[2], y[3]));
                 y[0] = u.x; y[1] = u.y; y[2] = w.x; y[3] = w.y;
             }
         }
@@ -460,7 +436,7 @@ attend_kernel(const Args a) {
                 uint32_t c[8] = {u0 & 0x000f000fu, u0 & 0x00f000f0u, u1 & 0x000f000fu, u1 & 0x00f000f0u, w0 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x000f000fu, w1 & 0x00f000f0u};
                 const uint32_t y0 = __byte_perm(mz[0][i >> 1], mz[1][i >> 1], half) & 0x000f000fu, y1 = __byte_perm(mz[2][i >> 1], mz[3][i >> 1], half) & 0x000f000fu;
 #pragma unroll
-                for (int k = 0; k < 8; ++k) c[k] = half2_less(c[k], (k & 2 ? y1 : y0) << (k & 1 ? 4 : 0));
+                for (int k = 0; k < 8; ++k) c[k] = q4_minus(c[k], (k & 2 ? y1 : y0) << (k & 1 ? 4 : 0));
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     const uint32_t b0 = transposed(h0[i - i0][n]), b1 = transposed(h1[i - i0][n]);

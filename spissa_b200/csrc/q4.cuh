@@ -31,6 +31,12 @@ __device__ __forceinline__ uint32_t q4_less(uint32_t c, uint32_t z) {
     return *(const uint32_t*)&r;
 }
 
+// the same by their first form: the bits in their places ARE the float16 numbers c · 2^-24 (16 c · 2^-24), and so are z's
+__device__ __forceinline__ uint32_t q4_minus(uint32_t c, uint32_t z) {
+    const __half2 r = __hsub2(*(const __half2*)&c, *(const __half2*)&z);
+    return *(const uint32_t*)&r;
+}
+
 __device__ __forceinline__ uint32_t bf2_sub(uint32_t a, uint32_t b) {
     const __nv_bfloat162 r = __hsub2(*(const __nv_bfloat162*)&a, *(const __nv_bfloat162*)&b);
     return *(const uint32_t*)&r;

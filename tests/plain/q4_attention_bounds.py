@@ -6,7 +6,7 @@ The bound of an output, from its terms. p_k: probabilities, v_k = s_k (c_k − z
   below the 24 bits of the largest (2^-23 of the sum of sizes each), and then one 32-bit sum a group: 70 · 2^-23 of the size of its
   terms; float32 queries are two float16 numbers, off by 2^-22 of an entry; the exponent's own product, rounding and 2^x: 4 · 2^-23 of
   the score and 2^-21.
-  ``size``: Σ |q| |k|, or for bfloat16 queries, whose products are with the codes and not with c − z, Σ |q| 15 s (1 + its use twice).
+  ``size``: Σ |q| |k|.
 * So a probability is off by e^δ − 1 of itself, in the sum over the keys and in the weighted one: 2 (e^δ − 1) Σ p |v|.
 * p s is one float16 number (2^-11 of itself) or two (2^-22), and no less than a smallest step off, which is 2^-33 of the largest
   p s that the group of columns has met (float32: 2^-44): a key's share of that times |c − z| <= 15.
@@ -29,9 +29,9 @@ def scales(x, group=32):
     return s[:, None].expand(-1, group).reshape(x.shape)
 
 
-def rows(q, k, v, sk, sv, first, scale, window=None, sink=None):
+def rows(q, k, v, sv, first, scale, window=None, sink=None):
     """(want, tolerance), each [n, nh, hd], for queries ``q`` [n, nh, hd] at positions first ..; ``k``, ``v`` [L, nkv, hd] float64:
-    what the codes stand for, ``sk``, ``sv`` their groups' scales."""
+    what the codes stand for, ``sv`` the values' groups' scales."""
     n, nh, hd = q.shape
     G, bf16 = nh // k.shape[1], q.dtype == torch.bfloat16
     want, tol = torch.zeros(n, nh, hd, dtype=F64), torch.zeros(n, nh, hd, dtype=F64)
@@ -41,7 +41,7 @@ def rows(q, k, v, sk, sv, first, scale, window=None, sink=None):
             ks, vs = k[lowest:p + 1, h // G], v[lowest:p + 1, h // G]
             x = q[i, h].to(F64)
             score = ks @ x * scale
-            size = (3 * 15 * sk[lowest:p + 1, h // G] if bf16 else ks.abs()) @ x.abs() * scale
+            size = ks.abs() @ x.abs() * scale
             top = score.max() if sink is None else torch.maximum(score.max(), sink[h].to(F64))
             w = torch.exp(score - top)
             w = w / (w.sum() + (torch.exp(sink[h].to(F64) - top) if sink is not None else 0.0))

@@ -20,7 +20,7 @@ def expected(q, kv, new, before, scale, window=None, sinks=None):
     """(want, tolerance) [tokens, nh · hd] of sequences with keys and values ``kv``."""
     parts, at = [], 0
     for (k, v), n, b in zip(kv, new, before):
-        parts.append(B.rows(q[at:at + n], Q.q4(k, 32), Q.q4(v, 32), B.scales(k), B.scales(v), b, scale, window, sinks))
+        parts.append(B.rows(q[at:at + n], Q.q4(k, 32), Q.q4(v, 32), B.scales(v), b, scale, window, sinks))
         at += n
     return tuple(torch.cat(x).reshape(at, -1) for x in zip(*parts))
 
@@ -108,6 +108,25 @@ def test_columns_of_zeros_stay_zeros(hd, dtype):
     for plan in (None, (1, 47, 1), (2, 10, 5)):
         out = attend(meta, pool, q, nh, nkv, hd, [1], None, None, plan)
         assert bool((out[0].cpu()[zero] == 0).all()) and bool((out[0].cpu()[~zero] != 0).all())
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_a_keys_large_entry_that_a_query_does_not_see_leaves_its_score_alone(hd, dtype):
+    """One channel of the keys is large and the queries are zero there; the others of its group stand for zeros, so every key's score comes
+    from the other groups."""
+    n, nh, nkv = 500, 4, 2
+    gen = torch.Generator().manual_seed(hd + 1)
+    q, k, v = (torch.randn(s, h, hd, generator=gen) for s, h in ((1, nh), (n, nkv), (n, nkv)))
+    k[..., 5] = 2.0 ** 17 * (1 + torch.rand(n, nkv, generator=gen))
+    k[..., 9] = -2.0 ** 16 * (1 + torch.rand(n, nkv, generator=gen))
+    q[..., 5] = q[..., 9] = 0.0
+    q = q.to(dtype)
+    want, tol = expected(q, [(k, v)], [1], [n - 1], 1.0 / math.sqrt(hd))
+    meta = KH.paged_meta([1], [n - 1], DEV)
+    pool = fill(meta, [(k, v)], nkv, hd)
+    for plan in (None, (1, 8, 1), (2, 8, 1)):
+        holds(attend(meta, pool, q, nh, nkv, hd, [1], None, None, plan), want, tol, plan)
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
