@@ -24,14 +24,8 @@ __device__ __forceinline__ uint32_t q4_pair(uint32_t word, int j) { return ((wor
 __device__ __forceinline__ float q4_scale_of(uint32_t meta) { return __uint_as_float((meta & 0xfff0u) << 16); }
 __device__ __forceinline__ float q4_value(int code, uint32_t meta) { return q4_scale_of(meta) * (float)(code - (int)(meta & 15u)); }
 
-// c − z as two float16 numbers, exactly, from the bits (w & 0x000f000f, or w & 0x00f000f0: 16 c) and z (16 z) in the same places
-__device__ __forceinline__ uint32_t q4_less(uint32_t c, uint32_t z) {
-    const uint32_t a = c | 0x64006400u, b = z | 0x64006400u;         // 1024 + c, 1024 + z
-    const __half2 r = __hsub2(*(const __half2*)&a, *(const __half2*)&b);
-    return *(const uint32_t*)&r;
-}
-
-// the same by their first form: the bits in their places ARE the float16 numbers c · 2^-24 (16 c · 2^-24), and so are z's
+// c − z as two float16 numbers, exactly: the bits in their places (w & 0x000f000f, or w & 0x00f000f0) ARE the float16 numbers c · 2^-24
+// (16 c · 2^-24), and so are z's
 __device__ __forceinline__ uint32_t q4_minus(uint32_t c, uint32_t z) {
     const __half2 r = __hsub2(*(const __half2*)&c, *(const __half2*)&z);
     return *(const uint32_t*)&r;

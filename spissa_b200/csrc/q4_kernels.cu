@@ -90,11 +90,14 @@ unpack_kernel(const uint4* codes, const uint16_t* meta, T* out, int rows, int K,
 // ARE the float16 c · 2^-24, one place up 16 c · 2^-24, so w & 0x000f000f and w & 0x00f000f0 are operands of m16n8k16, and w >> 8
 // holds the next two pairs (tensor cores take subnormal numbers as any other). (As e4m3 numbers a code is c · 2^-9 and takes
 // half of that, but m16n8k32 on those runs at half the rate of two on float16 here.)
+// The operands are c − z, differences of two such numbers, which are exact: tensor cores cut partial sums to 24 bits, and sums of x c are
+// many times those of x (c − z), which are nothing where weights are zeros beside a large one of their group. (With z Σ x taken off
+// afterwards a row of such zeros came to 2^-24 of the large one. us so / now: a row at 4096 x 14336 15.8 / 15.8, eight of gate and up of
+// 14336 x 4096 19.2 / 20.1, sixteen at 4096 x 14336 23.6 / 22.9; float32 rows, which met 1024 + c less 1024 + z, 21.0 / 19.0.)
 // x is multiplied by a power of two per row and block of 128 columns that brings the block's largest entry into 2^14 .. 2^15:
-// exact for bfloat16 entries down to 2^-26 of the block's largest, off by 2^-39 of the largest below. float32 entries are two
-// float16 numbers each, 22 bits, and meet c − z itself, as 1024 + c less 1024 + z: tensor cores cut partial sums to 24 bits
-// instead of rounding them, and sums of x c are many times those of x (c − z). (Blocks whose largest entry lies outside 2^-80 .. 2^100 overflow or vanish.) The zero is taken off
-// the sums, Σ x (c − z) = Σ x c − z Σ x, with Σ x per group in 32 bits, and a group's sum is scaled in 32 bits. A row with
+// exact for bfloat16 entries down to 2^-27 of the block's largest, off by 2^-35 of the largest below (every other pair of columns meets
+// 16 (c − z), and x / 16; the others: 2^-39). float32 entries are two float16 numbers each, 22 bits, which end at the same places.
+// (Blocks whose largest entry lies outside 2^-80 .. 2^100 overflow or vanish.) A group's sum is scaled in 32 bits. A row with
 // an entry that is not finite gives NaN.
 //
 // x stands still: a warp owns a block of columns, whose x it holds in registers as the operands want it, and walks over
@@ -102,9 +105,10 @@ unpack_kernel(const uint4* codes, const uint16_t* meta, T* out, int rows, int K,
 // would half fill, takes one partial sum a tile and block; warps of a CTA and CTAs of a cluster share K, and at the end
 // their sums are added in order: a row's result depends neither on timing nor on the other rows.
 //
-// Measured (us; 1, 8 and 16 bfloat16 rows, 8 float32 ones; weights in turns beyond L2): 4096 x 14336 15.6, 15.9, 23.6, 20.9; 4096 x 4096 6.8,
-// 7.2, 10.2, 8.3; 2 x 14336 x 4096 in groups of 128 18.9, 19.4, 48, 28. Up to 3.2 TB/s of codes, the arithmetic pipe at half its rate over
-// the launch. From 9 bfloat16 rows on all but small weights go to the tcgen05 cores (q4_tc.cu).
+// Measured (us; 1, 8 and 16 bfloat16 rows, 8 float32 ones; weights in turns beyond L2): 4096 x 14336 15.8, 16.4, 22.9, 19.0; 4096 x 4096 7.2,
+// 7.2, 10.0, 7.9; 2 x 14336 x 4096 in groups of 128 19.5, 20.1, 48.5, 25.3. Up to 3.1 TB/s of codes; over the launch the issue slots and
+// the arithmetic pipe are half used: a start and an end of some microseconds, and 16 warps an SM, are the rest. From 9 bfloat16 rows on
+// all but small weights go to the tcgen05 cores (q4_tc.cu).
 enum { MODE_STORE = 0, MODE_ACCUMULATE = 1, MODE_SILU_MUL = 2 };
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -209,7 +213,7 @@ gemv_kernel(const TX* x, const Product p) {
 
         // x of this block: lane (row g, columns 32 q + 8 t ..), eight rows at a time
         uint4 xv[NT][4][PARTS];
-        float2 by[NT], sx[NT][GROUPS];                               // of rows 2 t and 2 t + 1
+        float2 by[NT];                                               // of rows 2 t and 2 t + 1
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             const int token = n * 8 + g;
@@ -224,16 +228,14 @@ gemv_kernel(const TX* x, const Product p) {
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
             const int up = top > 0.0f ? min(94, max(-94, 141 - (int)(__float_as_uint(top) >> 23))) : 0;
-            const float scale = __uint_as_float((uint32_t)(127 + up) << 23), unit = __uint_as_float((uint32_t)((PARTS == 2 ? 127 : 151) - up) << 23);
+            const float scale = __uint_as_float((uint32_t)(127 + up) << 23), unit = __uint_as_float((uint32_t)(151 - up) << 23);
             by[n] = make_float2(__shfl_sync(0xffffffffu, unit, 8 * t), __shfl_sync(0xffffffffu, unit, 8 * t + 4));
-            float sum = 0.0f;
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 uint32_t h[PARTS][4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const float lo = v[q][2 * j] * scale, hi = v[q][2 * j + 1] * scale, f = j & 1 ? 0.0625f : 1.0f;
-                    sum += lo + hi;
                     h[0][j] = half2_of(lo * f, hi * f);
                     if (PARTS == 2) {
                         const float2 first = __half22float2(*(const __half2*)&h[0][j]);
@@ -242,13 +244,6 @@ gemv_kernel(const TX* x, const Product p) {
                 }
 #pragma unroll
                 for (int part = 0; part < PARTS; ++part) xv[n][q][part] = make_uint4(h[part][0], h[part][1], h[part][2], h[part][3]);
-                if ((q + 1) % (GROUP / 32) == 0) {
-                    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-                    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-                    sum *= -5.9604644775390625e-8f;                  // −2^-24 Σ x: in the units of the codes' products
-                    sx[n][q / (GROUP / 32)] = make_float2(__shfl_sync(0xffffffffu, sum, 8 * t), __shfl_sync(0xffffffffu, sum, 8 * t + 4));
-                    sum = 0.0f;
-                }
             }
         }
 
@@ -278,13 +273,11 @@ gemv_kernel(const TX* x, const Product p) {
                                 const uint4 c = w[d][r][q >> 1];
                                 const uint32_t r0 = (q & 1 ? c.y : c.x) >> (8 * half), r1 = (q & 1 ? c.w : c.z) >> (8 * half);
                                 uint32_t a0 = r0 & 0x000f000fu, a1 = r1 & 0x000f000fu, a2 = r0 & 0x00f000f0u, a3 = r1 & 0x00f000f0u;
-                                if (PARTS == 2) {
-                                    const uint32_t mm = m[d][r][q / (GROUP / 32)], z0 = (mm & 15u) * 0x10001u, z1 = ((mm >> 16) & 15u) * 0x10001u;
-                                    a0 = q4_less(a0, z0);
-                                    a1 = q4_less(a1, z1);
-                                    a2 = q4_less(a2, z0 << 4);
-                                    a3 = q4_less(a3, z1 << 4);
-                                }
+                                const uint32_t mm = m[d][r][q / (GROUP / 32)], z0 = (mm & 15u) * 0x10001u, z1 = ((mm >> 16) & 15u) * 0x10001u;
+                                a0 = q4_minus(a0, z0);
+                                a1 = q4_minus(a1, z1);
+                                a2 = q4_minus(a2, z0 << 4);
+                                a3 = q4_minus(a3, z1 << 4);
 #pragma unroll
                                 for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -299,20 +292,12 @@ gemv_kernel(const TX* x, const Product p) {
                             for (int r = 0; r < RT; ++r) {
                                 const uint32_t mm = m[d][r][i];
                                 const float s0 = __uint_as_float((mm << 16) & 0xfff00000u), s1 = __uint_as_float(mm & 0xfff00000u);
-                                const float z0 = PARTS == 2 ? 0.0f : (float)(mm & 15u), z1 = PARTS == 2 ? 0.0f : (float)((mm >> 16) & 15u);
 #pragma unroll
                                 for (int n = 0; n < NT; ++n) {
-                                    if (PARTS == 2) {
-                                        y[r][n].x = fmaf(s0, acc[r][n][0], y[r][n].x);
-                                        y[r][n].y = fmaf(s0, acc[r][n][1], y[r][n].y);
-                                        y[r][n].z = fmaf(s1, acc[r][n][2], y[r][n].z);
-                                        y[r][n].w = fmaf(s1, acc[r][n][3], y[r][n].w);
-                                        continue;
-                                    }
-                                    y[r][n].x = fmaf(s0, fmaf(z0, sx[n][i].x, acc[r][n][0]), y[r][n].x);
-                                    y[r][n].y = fmaf(s0, fmaf(z0, sx[n][i].y, acc[r][n][1]), y[r][n].y);
-                                    y[r][n].z = fmaf(s1, fmaf(z1, sx[n][i].x, acc[r][n][2]), y[r][n].z);
-                                    y[r][n].w = fmaf(s1, fmaf(z1, sx[n][i].y, acc[r][n][3]), y[r][n].w);
+                                    y[r][n].x = fmaf(s0, acc[r][n][0], y[r][n].x);
+                                    y[r][n].y = fmaf(s0, acc[r][n][1], y[r][n].y);
+                                    y[r][n].z = fmaf(s1, acc[r][n][2], y[r][n].z);
+                                    y[r][n].w = fmaf(s1, acc[r][n][3], y[r][n].w);
                                 }
                             }
                         }
