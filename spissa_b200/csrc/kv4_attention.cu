@@ -5,32 +5,34 @@
 // sees keys p − window + 1 .. p.
 //
 // The cache is read once per kv head and 8 NT columns, a column being a query head of a token. Codes are used as they lie: the
-// four bits in the lowest place of a half word ARE the float16 c · 2^-24, one place up 16 c · 2^-24, so an AND makes an operand
-// of mma.sync m16n8k16, with 16 keys (scores) or 16 columns of the values (output) as its rows and the query columns as
-// its columns: nothing is wasted on padding up to eight heads. Scales and zeros are applied to what is small:
+// four bits in the lowest place of a half word ARE the float16 c · 2^-24, one place up 16 c · 2^-24, so an AND and a multiplication
+// that takes the zero off (q4_minus) make an operand (c − z) 2^-9 of mma.sync m16n8k16, with 16 keys (scores) or 16 columns of the values
+// (output) as its rows and the query columns as its columns: nothing is wasted on padding up to eight heads. Scales are applied to
+// what is small:
 //   score  Σ_groups s Σ q' (c − z), q' = q times a power of two that brings a head's largest entry to 2^14: exact for bfloat16 entries
 //          down to 2^-27 of the largest, off by 2^-35 of the largest below; float32 as two such numbers, 22 bits;
 //   output Σ_keys (p s) (c − z): p s as a float16 number (off by 2^-11 of itself; float32: two, the second times 2^11, 2^-22), so that
 //          the scale s of a key's group of values costs no rounding of the values.
-// The operands are c − z, differences of two such numbers, which are exact: tensor cores cut partial sums to 24 bits, and sums of codes are
-// many times those of c − z, which are nothing where keys or values are zeros beside a large one of their group. (With z Σ q' and z Σ p s
-// taken off at the end a value of zero came to 2^-24 of 15 s a page, and a column's largest key to errors of the scores; the time is the
-// same.) With float32 queries a page's sums are added in 32 bits.
+// The operands are c − z: tensor cores cut partial sums to 24 bits, and sums of codes are many times those of c − z, which are nothing where
+// keys or values are zeros beside a large one of their group. (With z Σ q' and z Σ p s taken off at the end a value of zero came to 2^-24 of
+// 15 s a page, and a channel of large keys to errors of the scores.) With float32 queries a page's sums are added in 32 bits; 2,000 to
+// 30,000 keys are then 2.4e-7 off 64 bits, a plain evaluation in 32 bits 5 to 9e-7.
 // Two references, both moved in powers of two. A column's scores have one that follows the largest in steps: it moves only when a score
 // passes it by more than 2^8. And p s is multiplied by a power of two of its own for EVERY column and group of 32 columns of the values,
 // lowered (with the group's sums) when a product would pass float16: its largest then lies in 2^8 .. 2^9, so that p s is off by no
 // less than 2^-33 of the group's largest (float32: 2^-44), whatever other groups, heads or keys of little weight hold. When the scores'
 // reference rises by a factor, these rise with it, and the sums stay as they are. (One reference for the largest scale of any group and key
-// lost whole groups behind one large value; it took 50.3 us at 64 sequences of 2,048 keys where this takes 51.8, 46.2 / 47.5 for 40 tokens
-// behind 6,000, 221 / 257 for 2,000 float32 tokens.)
+// lost whole groups behind one large value; it took 50.5 us at 64 sequences of 2,048 keys where this takes 53.1, 46.5 / 48.4 for 40 tokens
+// behind 6,000, 221 / 251 for 2,000 float32 tokens of three prompts.)
 //
 // A page of a kv head is one run of bytes and arrives by one bulk copy in a ring; four warps take 16 of its keys each and keep
 // sums of their own, joined at the end in the order of the warps, then of the chunks: results do not depend on timing.
 // A key or value that is not finite reaches the columns that see it and no others.
 //
-// Measured (32 heads on 8 of 128, bfloat16): 64 sequences of 2,048 keys 50 us for 122 MB of pages, 2.4 TB/s; 3 of about 60,000 73;
-// 40 tokens behind 6,000 47; one sequence of 2,048 with heads of 64 10.7. Bound by instructions: some 470 a warp for 16 keys and eight
-// columns, with 57 % of the issue slots used at 64 sequences; more CTAs an SM (five of eight columns, three of sixteen) gain nothing.
+// Measured (32 heads on 8 of 128, bfloat16): 64 sequences of up to 2,048 keys 53 us for 122 MB of pages, 2.3 TB/s; 3 of about 50,000 76;
+// 40 tokens behind 6,000 48; one sequence of 2,048 with heads of 64 11. Some 470 instructions a warp for 16 keys and eight columns; no
+// pipe is full (issue slots 55 %, the arithmetic pipe 54 % at 64 sequences): latency at 16 warps an SM, a start and an end are the rest;
+// more CTAs an SM (five of eight columns, three of sixteen) gain nothing.
 #include "kv4.cuh"
 #include "async_copy.cuh"
 #include <cuda_fp16.h>
@@ -225,7 +227,7 @@ attend_kernel(const Args a) {
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         const int up = top > 0.0f ? min(94, max(-94, 141 - (int)(__float_as_uint(top) >> 23))) : 0;
-        const float by = __uint_as_float((uint32_t)(127 + up) << 23), back = __uint_as_float((uint32_t)(151 - up) << 23) * a.scale * LOG2E;
+        const float by = __uint_as_float((uint32_t)(127 + up) << 23), back = __uint_as_float((uint32_t)(136 - up) << 23) * a.scale * LOG2E;
 #pragma unroll
         for (int i = 0; i < NG; ++i) {
             uint32_t h[PARTS][4];
@@ -306,7 +308,7 @@ attend_kernel(const Args a) {
             uint32_t c[8] = {u0 & 0x000f000fu, u1 & 0x000f000fu, u0 & 0x00f000f0u, u1 & 0x00f000f0u, w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u};
             const uint32_t y0 = __byte_perm(km0[i >> 1], 0, i & 1 ? 0x3232 : 0x1010) & 0x000f000fu, y1 = __byte_perm(km1[i >> 1], 0, i & 1 ? 0x3232 : 0x1010) & 0x000f000fu;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) c[k] = q4_minus(c[k], (k & 1 ? y1 : y0) << (k & 2 ? 4 : 0));
+            for (int k = 0; k < 8; ++k) c[k] = q4_minus(c[k], q4_zero((k & 1 ? y1 : y0) << (k & 2 ? 4 : 0)));
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 float acc[4] = {0.f, 0.f, 0.f, 0.f};
@@ -436,7 +438,7 @@ attend_kernel(const Args a) {
                 uint32_t c[8] = {u0 & 0x000f000fu, u0 & 0x00f000f0u, u1 & 0x000f000fu, u1 & 0x00f000f0u, w0 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x000f000fu, w1 & 0x00f000f0u};
                 const uint32_t y0 = __byte_perm(mz[0][i >> 1], mz[1][i >> 1], half) & 0x000f000fu, y1 = __byte_perm(mz[2][i >> 1], mz[3][i >> 1], half) & 0x000f000fu;
 #pragma unroll
-                for (int k = 0; k < 8; ++k) c[k] = q4_minus(c[k], (k & 2 ? y1 : y0) << (k & 1 ? 4 : 0));
+                for (int k = 0; k < 8; ++k) c[k] = q4_minus(c[k], q4_zero((k & 2 ? y1 : y0) << (k & 1 ? 4 : 0)));
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     const uint32_t b0 = transposed(h0[i - i0][n]), b1 = transposed(h1[i - i0][n]);
@@ -496,7 +498,7 @@ attend_kernel(const Args a) {
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     const float back = __uint_as_float((254u << 23) - __float_as_uint(norm[n][i][e]));
-                    float2 v = make_float2(O[n][i][h][e] * (back * 16777216.0f), O[n][i][h][2 + e] * (back * 1048576.0f));
+                    float2 v = make_float2(O[n][i][h][e] * (back * 512.0f), O[n][i][h][2 + e] * (back * 32.0f));
                     if (poison[n] >> (2 * i + e) & 1) v.x = v.y = __int_as_float(0x7fc00000);
                     *(float2*)(acc + (warp * COLS + n * 8 + 2 * t + e) * ROW + 32 * i + 4 * g + 2 * h) = v;
                 }

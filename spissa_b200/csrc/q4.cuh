@@ -24,10 +24,15 @@ __device__ __forceinline__ uint32_t q4_pair(uint32_t word, int j) { return ((wor
 __device__ __forceinline__ float q4_scale_of(uint32_t meta) { return __uint_as_float((meta & 0xfff0u) << 16); }
 __device__ __forceinline__ float q4_value(int code, uint32_t meta) { return q4_scale_of(meta) * (float)(code - (int)(meta & 15u)); }
 
-// c − z as two float16 numbers, exactly: the bits in their places (w & 0x000f000f, or w & 0x00f000f0) ARE the float16 numbers c · 2^-24
-// (16 c · 2^-24), and so are z's
-__device__ __forceinline__ uint32_t q4_minus(uint32_t c, uint32_t z) {
-    const __half2 r = __hsub2(*(const __half2*)&c, *(const __half2*)&z);
+// (c − z) 2^-9 as two float16 numbers, exactly. The bits in their places (w & 0x000f000f, or w & 0x00f000f0) ARE the float16 numbers
+// c · 2^-24 (16 c · 2^-24), and so are z's; 2^15 makes ordinary numbers of them: tensor cores align a subnormal operand by the exponent it
+// is written with, and its product loses up to ten of the 24 bits (float32 products 3.5e-6 off where these are 2.4e-7).
+__device__ __forceinline__ uint32_t q4_zero(uint32_t z) {
+    const __half2 r = __hmul2(*(const __half2*)&z, __float2half2_rn(-32768.0f));
+    return *(const uint32_t*)&r;
+}
+__device__ __forceinline__ uint32_t q4_minus(uint32_t c, uint32_t zero) {
+    const __half2 r = __hfma2(*(const __half2*)&c, __float2half2_rn(32768.0f), *(const __half2*)&zero);
     return *(const uint32_t*)&r;
 }
 

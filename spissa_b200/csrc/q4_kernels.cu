@@ -87,13 +87,13 @@ unpack_kernel(const uint4* codes, const uint16_t* meta, T* out, int rows, int K,
 // ---------------------------------------------------------------- the product for a few tokens
 // out[M, N] = x[M, K] · Ŵ[N, K]ᵀ, M <= 16, bound by streaming the codes once; what stands in the way is instructions, so the
 // number type is the one that takes the fewest to pull a code out of its word: the four bits in the lowest place of a half word
-// ARE the float16 c · 2^-24, one place up 16 c · 2^-24, so w & 0x000f000f and w & 0x00f000f0 are operands of m16n8k16, and w >> 8
-// holds the next two pairs (tensor cores take subnormal numbers as any other). (As e4m3 numbers a code is c · 2^-9 and takes
-// half of that, but m16n8k32 on those runs at half the rate of two on float16 here.)
-// The operands are c − z, differences of two such numbers, which are exact: tensor cores cut partial sums to 24 bits, and sums of x c are
-// many times those of x (c − z), which are nothing where weights are zeros beside a large one of their group. (With z Σ x taken off
-// afterwards a row of such zeros came to 2^-24 of the large one. us so / now: a row at 4096 x 14336 15.8 / 15.8, eight of gate and up of
-// 14336 x 4096 19.2 / 20.1, sixteen at 4096 x 14336 23.6 / 22.9; float32 rows, which met 1024 + c less 1024 + z, 21.0 / 19.0.)
+// ARE the float16 c · 2^-24, one place up 16 c · 2^-24, so w & 0x000f000f and w & 0x00f000f0, a multiplication that takes the zero
+// off (q4_minus), are operands (c − z) 2^-9 of m16n8k16, and w >> 8 holds the next two pairs. (As e4m3 numbers a code is c · 2^-9 and
+// takes half of that, but m16n8k32 on those runs at half the rate of two on float16 here.)
+// Why c − z: tensor cores cut partial sums to 24 bits, and sums of x c are many times those of x (c − z), which are nothing where
+// weights are zeros beside a large one of their group. (With z Σ x taken off
+// afterwards a row of such zeros came to 2^-24 of the large one. us so / now: a row at 4096 x 14336 15.8 / 16.1, eight of gate and up of
+// 14336 x 4096 19.0 / 20.3, sixteen at 4096 x 14336 23.6 / 23.6; float32 rows, which met 1024 + c less 1024 + z, 20.9 / 19.5.)
 // x is multiplied by a power of two per row and block of 128 columns that brings the block's largest entry into 2^14 .. 2^15:
 // exact for bfloat16 entries down to 2^-27 of the block's largest, off by 2^-35 of the largest below (every other pair of columns meets
 // 16 (c − z), and x / 16; the others: 2^-39). float32 entries are two float16 numbers each, 22 bits, which end at the same places.
@@ -105,8 +105,8 @@ unpack_kernel(const uint4* codes, const uint16_t* meta, T* out, int rows, int K,
 // would half fill, takes one partial sum a tile and block; warps of a CTA and CTAs of a cluster share K, and at the end
 // their sums are added in order: a row's result depends neither on timing nor on the other rows.
 //
-// Measured (us; 1, 8 and 16 bfloat16 rows, 8 float32 ones; weights in turns beyond L2): 4096 x 14336 15.8, 16.4, 22.9, 19.0; 4096 x 4096 7.2,
-// 7.2, 10.0, 7.9; 2 x 14336 x 4096 in groups of 128 19.5, 20.1, 48.5, 25.3. Up to 3.1 TB/s of codes; over the launch the issue slots and
+// Measured (us; 1, 8 and 16 bfloat16 rows, 8 float32 ones; weights in turns beyond L2): 4096 x 14336 16.1, 16.4, 23.6, 19.5; 4096 x 4096 7.2,
+// 7.6, 10.0, 7.9; 2 x 14336 x 4096 in groups of 128 19.5, 20.3, 48.5, 25.3. Up to 3.1 TB/s of codes; over the launch the issue slots and
 // the arithmetic pipe are half used: a start and an end of some microseconds, and 16 warps an SM, are the rest. From 9 bfloat16 rows on
 // all but small weights go to the tcgen05 cores (q4_tc.cu).
 enum { MODE_STORE = 0, MODE_ACCUMULATE = 1, MODE_SILU_MUL = 2 };
@@ -228,7 +228,7 @@ gemv_kernel(const TX* x, const Product p) {
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
             const int up = top > 0.0f ? min(94, max(-94, 141 - (int)(__float_as_uint(top) >> 23))) : 0;
-            const float scale = __uint_as_float((uint32_t)(127 + up) << 23), unit = __uint_as_float((uint32_t)(151 - up) << 23);
+            const float scale = __uint_as_float((uint32_t)(127 + up) << 23), unit = __uint_as_float((uint32_t)(136 - up) << 23);
             by[n] = make_float2(__shfl_sync(0xffffffffu, unit, 8 * t), __shfl_sync(0xffffffffu, unit, 8 * t + 4));
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
@@ -274,10 +274,11 @@ gemv_kernel(const TX* x, const Product p) {
                                 const uint32_t r0 = (q & 1 ? c.y : c.x) >> (8 * half), r1 = (q & 1 ? c.w : c.z) >> (8 * half);
                                 uint32_t a0 = r0 & 0x000f000fu, a1 = r1 & 0x000f000fu, a2 = r0 & 0x00f000f0u, a3 = r1 & 0x00f000f0u;
                                 const uint32_t mm = m[d][r][q / (GROUP / 32)], z0 = (mm & 15u) * 0x10001u, z1 = ((mm >> 16) & 15u) * 0x10001u;
-                                a0 = q4_minus(a0, z0);
-                                a1 = q4_minus(a1, z1);
-                                a2 = q4_minus(a2, z0 << 4);
-                                a3 = q4_minus(a3, z1 << 4);
+                                const uint32_t n0 = q4_zero(z0), n1 = q4_zero(z1), n2 = q4_zero(z0 << 4), n3 = q4_zero(z1 << 4);
+                                a0 = q4_minus(a0, n0);
+                                a1 = q4_minus(a1, n1);
+                                a2 = q4_minus(a2, n2);
+                                a3 = q4_minus(a3, n3);
 #pragma unroll
                                 for (int n = 0; n < NT; ++n)
 #pragma unroll
