@@ -30,8 +30,8 @@
 // A key or value that is not finite reaches the columns that see it and no others.
 //
 // Measured (32 heads on 8 of 128, bfloat16): 64 sequences of up to 2,048 keys 53 us for 122 MB of pages, 2.3 TB/s; 3 of about 50,000 76;
-// 40 tokens behind 6,000 48; one sequence of 2,048 with heads of 64 11. Some 470 instructions a warp for 16 keys and eight columns; no
-// pipe is full (issue slots 55 %, the arithmetic pipe 54 % at 64 sequences): latency at 16 warps an SM, a start and an end are the rest;
+// 40 tokens behind 6,000 48; one sequence of 2,048 with heads of 64 11. Some 530 instructions a warp for 16 keys and eight columns; no
+// pipe is full (issue slots 60 %, the arithmetic pipe 53 % at 64 sequences): latency at 16 warps an SM, a start and an end are the rest;
 // more CTAs an SM (five of eight columns, three of sixteen) gain nothing.
 #include "kv4.cuh"
 #include "async_copy.cuh"

@@ -45,7 +45,8 @@ __host__ __device__ __forceinline__ int store_shift(int units) { return units <=
 
 // The angles are formed and their sine and cosine taken in 64 bits, keys are rotated in 64 bits and rounded to 32 once: at position
 // 100,000 an angle in 32 bits is off by up to 0.004, and a key's code is a comparison that an error of the rotation may turn.
-// 2,000 tokens of 32 + 2 x 8 heads of 128: 22.9 us for 68 MB (without rotation 20.6); 8 tokens 3.3. Bound by latency: a block's sines, rows
+// 2,000 tokens of 32 + 2 x 8 heads of 128: 26.2 us for 68 MB with rows from memory (without rotation 23.6), 19.6 with rows that L2 holds
+// (17.3); 8 tokens 3.6. Bound by latency: a block's sines, rows
 // in, a group's bounds by shuffles, codes out, at four blocks an SM. Eight columns a thread, more blocks an SM, rows prefetched
 // while the sines are formed: within 7 % either way.
 template <typename TQ, int NG>
@@ -183,7 +184,7 @@ __device__ __forceinline__ float4 read_quad(const uint8_t* tile, int slot, int d
     return make_float4(q4_value(w & 15, m), q4_value((w >> 16) & 15, m), q4_value((w >> 4) & 15, m), q4_value((w >> 20) & 15, m));
 }
 
-// 2,000 tokens of 8 kv heads of 128: 8.4 us, two and four bytes a read.
+// 2,000 tokens of 8 kv heads of 128: 8.7 us, two and four bytes a read.
 template <typename T>
 __global__ void __launch_bounds__(256)
 load_kernel(const uint8_t* pool, T* k_out, T* v_out, Place place, int nkv, int hd) {

@@ -106,8 +106,8 @@ unpack_kernel(const uint4* codes, const uint16_t* meta, T* out, int rows, int K,
 // their sums are added in order: a row's result depends neither on timing nor on the other rows.
 //
 // Measured (us; 1, 8 and 16 bfloat16 rows, 8 float32 ones; weights in turns beyond L2): 4096 x 14336 16.1, 16.4, 23.6, 19.5; 4096 x 4096 7.2,
-// 7.6, 10.0, 7.9; 2 x 14336 x 4096 in groups of 128 19.5, 20.3, 48.5, 25.3. Up to 3.1 TB/s of codes; over the launch the issue slots and
-// the arithmetic pipe are half used: a start and an end of some microseconds, and 16 warps an SM, are the rest. From 9 bfloat16 rows on
+// 7.6, 10.0, 7.9; 2 x 14336 x 4096 in groups of 128 19.5, 20.3, 48.5, 25.3. Up to 3.1 TB/s of codes; over the launch 57 % of the issue
+// slots and half of the arithmetic pipe are used: a start and an end of some microseconds, and 16 warps an SM, are the rest. From 9 bfloat16 rows on
 // all but small weights go to the tcgen05 cores (q4_tc.cu).
 enum { MODE_STORE = 0, MODE_ACCUMULATE = 1, MODE_SILU_MUL = 2 };
 

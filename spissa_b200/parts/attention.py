@@ -234,7 +234,7 @@ def reads_codes(q, cols: int, nkv: int, hd: int = 128, n_seqs: int = 1) -> bool:
       32 on 8 of 64, behind 2,000: 192 41/47, 256 65/36;    32 on 8 of 96: 192 77/57, 512 161/62;    32 on 8 of 32: 192 31/33, 512 66/44;
       9 on 3 of 96, behind 2,000: 256 29/55, 512 46/60, 1,024 96/69; behind 100,000: 256 748/2,316;    12 on 12 of 96: 384 45/61, 512 82/64;
       16 on 1 of 128, behind 2,000: 256 50/53, 512 100/57;    6 on 2 of 32: 512 24/36, 1,024 40/42; behind 100,000: 512 548/1,129;
-    1,024 tokens of 64 sequences behind 1,000 (32 on 8 of 128): 180/283; float32: 512 tokens behind nothing 66/146, behind 2,000 256/960."""
+    1,024 tokens of 64 sequences behind 1,000 (32 on 8 of 128): 180/283; float32: 512 tokens behind nothing 63/146, behind 2,000 254/960."""
     if q.dtype == torch.float32:
         return nkv * -(-cols // 16) < 1 << 16            # (tiles of columns are a grid's second dimension)
     return q.shape[0] < FLASH_TC_TOKENS or cols <= SPLIT4_COLUMNS or n_seqs * nkv * -(-cols // 16) <= K.kv4_room(hd)

@@ -155,8 +155,9 @@ class GatedLinear:
 
 class Linear4:
     """y = x · Ŵᵀ, Ŵ the numbers that ``weight`` [out, in] becomes in four bits, in groups of ``group`` (32, 64 or 128) columns;
-    in a multiple of the group. Called as ``Linear``: x bfloat16 or float32. Up to 16 rows stream the codes, some dozens of bfloat16
-    rows multiply with them on the tcgen05 cores, more (and float32 ones) unpack the weight first."""
+    in a multiple of the group. Called as ``Linear``: x bfloat16 or float32. Up to 16 rows stream the codes (from 9 bfloat16 rows on only
+    of small weights), up to 1,024 bfloat16 rows multiply with them on the tcgen05 cores where that is estimated to be the faster way
+    (``product4``), more, and float32 ones from 17 on, unpack the weight first."""
 
     def __init__(self, weight: torch.Tensor, group: int = 64):
         if weight.dim() != 2:
