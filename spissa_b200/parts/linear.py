@@ -192,7 +192,7 @@ class Linear4:
             return out
         way, mode = product4(self, x, self.out_features), K.TC_ACCUMULATE if accumulate else K.TC_STORE
         if way == "unpack":
-            return Linear(self.unpacked(x.dtype))(on_boundaries(x, 32), out=out, accumulate=accumulate)
+            return Linear(self.unpacked(x.dtype))(on_boundaries(x, 8), out=out, accumulate=accumulate)
         (K.q4_gemv if way == "gemv" else K.q4_tc)(on_boundaries(x), self.codes, self.scales, out, self.out_features, self.group, 0, mode)
         return out
 
@@ -227,7 +227,7 @@ class GatedLinear4:
             return out
         way = product4(self, x, 2 * self.intermediate, self.intermediate)
         if way == "unpack":
-            return self.unpacked(x.dtype)(on_boundaries(x, 32), act_dtype)
+            return self.unpacked(x.dtype)(on_boundaries(x, 8), act_dtype)
         (K.q4_gemv if way == "gemv" else K.q4_tc)(on_boundaries(x), self.codes, self.scales, out, 2 * self.intermediate, self.group,
                                                   self.intermediate, K.TC_SILU_MUL, self.act, self.mult)
         return out
@@ -283,10 +283,12 @@ def check4(lin, x, out, out_features: int, accumulate: bool) -> int:
     return x.shape[0]
 
 
-def on_boundaries(x, size: int = 16):
-    """``x``, or a copy of it where its rows do not start on boundaries of ``size`` bytes (columns of wider rows, an odd offset) or overlap
-    (one row for all): the tensor-core kernels take no such rows (16 bytes, the 32-bit one 32), and what does is the FFMA product
-    (2,048 bfloat16 rows of 4096 x 4096, us: 3,100, with the copy 86; 200 float32 ones 590 and 92)."""
+def on_boundaries(x, entries: int = 0):
+    """``x``, or a copy of it where its rows do not start on boundaries of 16 bytes, or of ``entries`` numbers where those are more
+    (columns of wider rows, an odd offset), or overlap (one row for all): the tensor-core kernels take no such rows (the 32-bit one wants
+    8 numbers), and what does is the FFMA product (2,048 bfloat16 rows of 4096 x 4096, us: 3,100, with the copy 86; 200 float32
+    ones 590 and 92)."""
+    size = max(16, entries * x.element_size())
     if (x.data_ptr() | x.stride(0) * x.element_size()) % size == 0 and x.stride(0) >= x.shape[1]:
         return x
     return x.clone(memory_format=torch.contiguous_format)

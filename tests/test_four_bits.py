@@ -163,3 +163,15 @@ def test_which_prompt_steps_read_the_codes():
                                  (1024, 6, 2, 32, True), (384, 16, 4, 32, True), (512, 16, 4, 32, False), (256, 32, 8, 64, False)):
         assert takes(T, 1, T, nh, nkv, hd) is want, (T, nh, nkv, hd)
     assert takes(1024, 64, 24, 32, 8, 128) and not takes(2048, 16, 128, 32, 8, 128) and not takes(2000, 3, 900, 32, 8, 128)
+
+
+def test_rows_are_copied_only_where_a_kernel_does_not_take_them():
+    from spissa_b200.parts.linear import on_boundaries
+    for dtype, entries, kept in ((torch.bfloat16, 8, (0, 8, 16)), (torch.bfloat16, 0, (0, 8, 16)), (torch.float32, 8, (0, 8, 16)), (torch.float32, 0, (0, 4, 8, 12))):
+        wide = torch.zeros(5, 96, dtype=dtype)
+        wide = wide[:, (-wide.data_ptr() // wide.element_size()) % 16:][:, :80]
+        for at in range(17):
+            rows = wide[:, at:at + 64]
+            assert (on_boundaries(rows, entries) is rows) == (at in kept or at % 16 == 0), (dtype, entries, at)
+    row = torch.zeros(1, 64)
+    assert on_boundaries(row.expand(5, 64)).is_contiguous() and on_boundaries(row) is row
