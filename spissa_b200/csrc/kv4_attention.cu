@@ -161,7 +161,7 @@ attend_kernel(const Args a) {
     constexpr bool Q_HELD = NT == 1 && PARTS == 1;                   // the queries' operands in registers, else in shared memory
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES];
-    __shared__ int failed;
+    __shared__ int failed, fetched;
     __shared__ float ref_s[WARPS][COLS], sum_s[WARPS][COLS];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int seq = blockIdx.z, kvh = blockIdx.y % a.nkv, tile = blockIdx.y / a.nkv, chunk = blockIdx.x, G = a.nh / a.nkv;
@@ -179,7 +179,7 @@ attend_kernel(const Args a) {
     const uint32_t ring = smem_u32(smem), q_at = ring + STAGES * TILE;
 
     if (threadIdx.x == 0) {
-        failed = 0;
+        failed = fetched = 0;
         for (int s = 0; s < STAGES; ++s) {
             mbar_init(smem_u32(&full[s]), 1);
             mbar_init(smem_u32(&empty[s]), WARPS);
@@ -194,6 +194,7 @@ attend_kernel(const Args a) {
     auto fetch = [&](int i, int page) {                              // one thread
         const int s = i % STAGES;
         mbar_expect_tx(smem_u32(&full[s]), TILE);
+        fetched = i + 1;
         bulk_copy_g2s(ring + s * TILE, a.pool + ((size_t)page * a.nkv + kvh) * TILE, TILE, smem_u32(&full[s]));
     };
     if (warp == 0) {
@@ -477,6 +478,12 @@ attend_kernel(const Args a) {
 
     // each warp's sums over its lanes, its columns' numbers in shared memory (where the pages were); then the warps', in their order
     __syncthreads();
+    if (failed) {                                                    // a wait ran out: copies may still be on their way into this CTA's memory
+        if (threadIdx.x == 0)
+            for (int i = max(0, fetched - STAGES); i < fetched; ++i) mbar_wait(smem_u32(&full[i % STAGES]), (i / STAGES) & 1, nullptr, 0);
+        __syncthreads();
+        return;
+    }
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -504,7 +511,6 @@ attend_kernel(const Args a) {
                 }
     }
     __syncthreads();
-    if (failed) return;
     for (int c = warp; c < n_cols; c += WARPS) {
         float big = ref_s[0][c], total = 0.0f, f[WARPS];
 #pragma unroll

@@ -93,7 +93,7 @@ q4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ 
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t bar_full[MAX_STAGES], bar_empty[MAX_STAGES], bar_a[MAX_SLOTS], bar_used[MAX_SLOTS], bar_acc;
     __shared__ uint32_t tmem_slot;
-    __shared__ int failed;
+    __shared__ int failed, asked;                                    // a wait ran out; stages that copies were asked for
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int row_tile = blockIdx.x / a.pieces, piece = blockIdx.x % a.pieces;
@@ -112,7 +112,7 @@ q4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ 
             mbar_init(smem_u32(&bar_used[s]), 1);
         }
         mbar_init(smem_u32(&bar_acc), 1);
-        failed = 0;
+        failed = asked = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -133,6 +133,7 @@ q4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ 
             for (int b = b0; b < b1; ++b) {
                 if (!wait_for(smem_u32(&bar_empty[s]), ph, a.status, 181, &failed)) break;
                 const uint32_t to = base + (uint32_t)s * stage_bytes, bar = smem_u32(&bar_full[s]);
+                asked = b - b0 + 1;
                 mbar_expect_tx(bar, stage_bytes_in);
                 tma_load_4d(to + x_bytes, &map_codes, 0, 0, b, row_tile * TILES, bar);
                 tma_load_3d(to + x_bytes + TILES * 1024, &map_meta, 0, b, row_tile * TILES, bar);
@@ -224,6 +225,8 @@ q4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ 
     // its own cluster on the same SM, or from a cluster of another stream that holds what this one's other CTAs wait for.
     tc_fence_before();
     __syncthreads();
+    if (failed && threadIdx.x == 0)                                  // copies may still be on their way into this CTA's memory
+        for (int i = max(0, asked - a.stages); i < asked; ++i) mbar_wait(smem_u32(&bar_full[i % a.stages]), (uint32_t)(i / a.stages) & 1u, nullptr, 0);
     if (warp == 1) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(a.tmem_cols) : "memory");
