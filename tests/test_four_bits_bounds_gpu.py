@@ -34,7 +34,7 @@ def holds(out, want, tol, note=""):
 @pytest.mark.parametrize("kind", ["q", "p"])
 @pytest.mark.parametrize("hd", [64, 128])
 def test_float32_needs_both_parts(kind, hd):
-    """The cases whose bound a single float16 part of the queries, or of p s, passes."""
+    """The cases whose bound a single float16 part of the queries, or of p s, would exceed."""
     q, k, v = aligned_case(kind, hd)
     n = k.shape[0]
     for G in (1, 5):                                                 # eight columns a CTA, whatever is in them
